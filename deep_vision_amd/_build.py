@@ -68,6 +68,9 @@ def _compile(src: str, debug: bool) -> str:
         "hipcc", f"--offload-arch={ARCH}", "-std=c++17", "-fPIC", *flags, "-c", src, "-o", obj,
         f"-I{CSRC}", f"-I{pybind11.get_include()}", f"-I{sysconfig.get_paths()['include']}",
         "-Wno-unused-result", "-Wno-unused-value",
+        # no packed fp32 instructions (v_pk_add / mul / fma_f32): hipcc -O3 forms them from plain float
+        # code, and some of their forms have given wrong results now and then on this hardware
+        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     ]
     if debug:
         cmd.append("-DDV_DEBUG=1")
