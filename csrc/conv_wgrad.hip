@@ -620,7 +620,7 @@ int dv_conv_wgrad(const ConvWgradArgs& a, hipStream_t st) {
     p.atomic_out = 0;
     p.accumulate = 0;
   } else if (p.atomic_out && !a.accumulate) {
-    (void)hipMemsetAsync(a.dw, 0, out_elems * sizeof(float), st);
+    dv_zero(a.dw, (int64_t)out_elems, st);
   }
   // plain rows: the im2col of a 1x1 / stride-1 / pad-0 conv is X itself (pixel grid == input grid)
   const bool plain = a.R == 1 && a.S == 1 && a.sh == 1 && a.sw == 1 && a.ph == 0 && a.pw == 0 && a.P == a.H &&

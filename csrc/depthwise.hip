@@ -1273,7 +1273,7 @@ int dv_dw_wgrad(const void* x, const void* dy, float* dw, int N, int H, int W, i
                 int K, int sh, int sw, int ph, int pw, int accumulate, hipStream_t st) {
   if (!dw_shape_ok(C, ldx, ldy) || (sw != 1 && sw != 2)) return -1;
   DwGeo g{N, H, W, C, ldx, P, Q, ldy, sh, sw, ph, pw, {}, {}};
-  if (!accumulate) (void)hipMemsetAsync(dw, 0, (size_t)C * K * K * sizeof(float), st);
+  if (!accumulate) dv_zero(dw, (int64_t)C * K * K, st);
   if (sw == 1) {
     DW_KS(K, (wgrad_variants<KS, 1>(x, dy, dw, g, st)))
   } else {

@@ -240,6 +240,8 @@ void dv_rmsprop(float* p, const float* g, float* sq, float* mom, float* gavg, in
                 const float* skip = nullptr);
 void dv_nonfinite_check(const float* g, int64_t n, float* guard, hipStream_t st);
 void dv_nonfinite_tally(float* guard, hipStream_t st);
+// x = 0 by a kernel: memset nodes of a captured graph have given wrong results on later replays
+void dv_zero(float* x, int64_t n, hipStream_t st);
 void dv_sumsq(const float* x, int64_t n, float* out, hipStream_t st);
 
 // ---- depthwise conv (depthwise.hip) ----

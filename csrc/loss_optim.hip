@@ -233,6 +233,12 @@ void dv_nonfinite_check(const float* g, int64_t n, float* guard, hipStream_t st)
   else nonfinite_check_kernel<false><<<std::min(grid_for(n), 1024), NT, 0, st>>>(g, n, guard);
 }
 void dv_nonfinite_tally(float* guard, hipStream_t st) { nonfinite_tally_kernel<<<1, 1, 0, st>>>(guard); }
+__global__ __launch_bounds__(NT) void zero_kernel(float* __restrict__ x, int64_t n) {
+  for (int64_t i = blockIdx.x * (int64_t)NT + threadIdx.x; i < n; i += (int64_t)gridDim.x * NT) x[i] = 0.f;
+}
+void dv_zero(float* x, int64_t n, hipStream_t st) {
+  if (n > 0) zero_kernel<<<grid_for(n), NT, 0, st>>>(x, n);
+}
 void dv_sumsq(const float* x, int64_t n, float* out, hipStream_t st) {
   const int grid = std::min(grid_for(n), 1024);
   float* det = dv_deterministic() ? dv_det_workspace((size_t)grid, st) : nullptr;
