@@ -353,16 +353,14 @@ def main():
 
     import contextlib
 
-    # eager steps run on a high-priority stream of their own, so the weight-gradient side stream
-    # (normal priority) soaks up the CUs the main path leaves idle instead of competing for them:
-    # ResNet-50 13,936 -> 14,017 / 14,044 img/s, same box, two pairs (profiles/main_stream_priority_ab.txt).
-    # DV_MAIN_PRIO=0 keeps the default stream.
-    prio = contextlib.nullcontext()
-    if cuda and os.environ.get("DV_MAIN_PRIO", "1") == "1" and not args.graph:
-        main_stream = torch.cuda.Stream(device=device, priority=-1)
+    # eager steps run on a stream of their own beside the weight-gradient side stream, at the same
+    # (default) priority: work on streams of different priorities can hang this hardware
+    own_stream = contextlib.nullcontext()
+    if cuda and not args.graph:
+        main_stream = torch.cuda.Stream(device=device)
         main_stream.wait_stream(torch.cuda.current_stream(device))
-        prio = torch.cuda.stream(main_stream)
-    with prio:
+        own_stream = torch.cuda.stream(main_stream)
+    with own_stream:
         for _ in range(args.warmup):
             loss = step()
         sync()
