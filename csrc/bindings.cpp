@@ -344,6 +344,39 @@ PYBIND11_MODULE(_C, m) {
     if (dv_lrn_bwd(CP(x), CP(dy), P(dx), npix, C, lo, hi, alpha, beta, k, ST(st))) throw std::runtime_error("lrn_bwd: C > 1024");
     check_last("lrn_bwd");
   });
+  m.def("adamw32", [](uptr p, uptr g, uptr m_, uptr v, int64_t n, float lr, double b1, double b2, float eps, float wd,
+                      double bc1, double bc2, float gscale, uptr hp, uptr skip, uptr st) {
+    const DvAdamW a{lr, wd, (float)b1, (float)(1 - b1), (float)b2, (float)(1 - b2), eps, (float)bc1, (float)bc2, gscale,
+                    0, 0, CFP(hp), CFP(skip)};
+    if (dv_adamw32(a, FP(p), CFP(g), FP(m_), FP(v), n, ST(st))) throw std::runtime_error("adamw32: unsupported length");
+    check_last("adamw32");
+  });
+  m.def("adamw8", [](uptr p, uptr g, uptr m8, uptr ms, uptr r8, uptr rs, uptr chunks, int nchunks, float lr, double b1,
+                     double b2, float eps, float wd, double bc1, double bc2, float gscale, uint32_t step, uint32_t seed,
+                     uptr hp, uptr skip, uptr st) {
+    const DvAdamW a{lr, wd, (float)b1, (float)(1 - b1), (float)b2, (float)(1 - b2), eps, (float)bc1, (float)bc2, gscale,
+                    step, seed, CFP(hp), CFP(skip)};
+    if (dv_adamw8(a, CP(chunks), nchunks, FP(p), CFP(g), reinterpret_cast<uint8_t*>(m8), FP(ms),
+                  reinterpret_cast<uint8_t*>(r8), FP(rs), ST(st)))
+      throw std::runtime_error("adamw8: no chunks");
+    check_last("adamw8");
+  });
+  m.attr("ADAMW_BLOCK") = DV_ADAMW_BLOCK;
+  m.attr("ADAMW_CHUNK") = DV_ADAMW_CHUNK;
+  m.def("layer_norm_parts", [](int bf16, int64_t rows, int D) { return dv_layer_norm_parts(bf16, rows, D); });
+  m.def("layer_norm_fwd", [](uptr x, int bf16, int64_t ldx, uptr w, uptr b, uptr y, uptr stats, int64_t rows, int D,
+                             float eps, uptr st) {
+    if (dv_layer_norm_fwd(CP(x), bf16, ldx, CFP(w), CFP(b), P(y), FP(stats), rows, D, eps, ST(st)))
+      throw std::runtime_error("layer_norm_fwd: unsupported shape");
+    check_last("layer_norm_fwd");
+  });
+  m.def("layer_norm_bwd", [](uptr x, int bf16, int64_t ldx, uptr dy, int64_t ldg, uptr w, uptr stats, uptr dx, uptr part,
+                             int parts, uptr dw, uptr db, int acc_w, int acc_b, int64_t rows, int D, uptr st) {
+    if (dv_layer_norm_bwd(CP(x), bf16, ldx, CP(dy), ldg, CFP(w), CFP(stats), P(dx), FP(part), parts, FP(dw), FP(db),
+                          acc_w, acc_b, rows, D, ST(st)))
+      throw std::runtime_error("layer_norm_bwd: unsupported shape");
+    check_last("layer_norm_bwd");
+  });
   m.def("sumsq", [](uptr x, int64_t n, uptr out, uptr st) { dv_sumsq(CFP(x), n, FP(out), ST(st)); check_last("sumsq"); });
 
   m.def("channel_sum_finalize", [](uptr acc, int ld, int C, uptr out, int accumulate, uptr st) {

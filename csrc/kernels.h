@@ -240,6 +240,34 @@ void dv_rmsprop(float* p, const float* g, float* sq, float* mom, float* gavg, in
                 const float* skip = nullptr);
 void dv_nonfinite_check(const float* g, int64_t n, float* guard, hipStream_t st);
 void dv_nonfinite_tally(float* guard, hipStream_t st);
+// ---- AdamW (adamw.hip) ----
+constexpr int DV_ADAMW_BLOCK = 256;   // values that share the scale of their 8-bit moments
+constexpr int DV_ADAMW_CHUNK = 4096;  // values of one tensor a workgroup updates
+struct DvAdamW {
+  float lr, wd, b1, omb1, b2, omb2, eps, bc1, bc2, gscale;
+  uint32_t step, seed;
+  const float* hp;    // device [lr, bc1, bc2, step] of a captured step, or null
+  const float* skip;  // device non-finite guard, or null
+};
+struct DvAdamWChunk {
+  int64_t first;  // its first value in the flat parameter / gradient buffers
+  int64_t block;  // its first block of the moments
+  int64_t n;      // values, at most DV_ADAMW_CHUNK
+};
+int dv_adamw32(const DvAdamW& a, float* p, const float* g, float* m, float* v, int64_t n, hipStream_t st);
+int dv_adamw8(const DvAdamW& a, const void* chunks, int nchunks, float* p, const float* g, uint8_t* m8, float* ms,
+              uint8_t* r8, float* rs, hipStream_t st);
+
+// ---- layer norm (layer_norm.hip) ----
+// x / dy rows at strides ldx / ldg, y / dx dense; stats [rows][2] = mean, rstd; w / b / dw / db may be null.
+// part: [parts][2][D] scratch with parts = dv_layer_norm_parts(); acc_w / acc_b add into dw / db.
+int dv_layer_norm_parts(int is_bf16, int64_t rows, int D);
+int dv_layer_norm_fwd(const void* x, int is_bf16, int64_t ldx, const float* w, const float* b, void* y, float* stats,
+                      int64_t rows, int D, float eps, hipStream_t st);
+int dv_layer_norm_bwd(const void* x, int is_bf16, int64_t ldx, const void* dy, int64_t ldg, const float* w,
+                      const float* stats, void* dx, float* part, int parts, float* dw, float* db, int acc_w, int acc_b,
+                      int64_t rows, int D, hipStream_t st);
+
 // x = 0 by a kernel: memset nodes of a captured graph have given wrong results on later replays
 void dv_zero(float* x, int64_t n, hipStream_t st);
 void dv_sumsq(const float* x, int64_t n, float* out, hipStream_t st);

@@ -1,0 +1,398 @@
+// Layer norm over the last dimension, forward and backward.
+//
+//   mu = mean(x), rstd = 1 / sqrt(mean((x - mu)^2) + eps), xh = (x - mu) * rstd, y = w * xh + b
+//   h = dy * w,  dx = rstd * (h - mean(h) - xh * mean(h * xh)),  dw = sum_rows dy * xh,  db = sum_rows dy
+//
+// Bound by memory: forward reads x and writes y once, backward reads x and dy and writes dx once.
+// A row stays in the registers of its LANES lanes (16 bytes a load, VECS loads a lane), so the
+// variance is summed over (x - mu) itself, in fp32 and without cancellation. Each lane owns the
+// same columns of every row it visits: w and b are loaded once a block, and the sums for dw / db
+// stay in registers until the block's last row. Those partial sums go to a [block][2][D] slab that
+// a second launch folds in a fixed order: no atomics, the same bits every time.
+//
+// Rows may be slices of wider ones (row stride ldx / ldg) and start at any element: 16-byte loads of
+// global memory need no alignment on this hardware. D is padded to whole vectors per lane by
+// masking, the last vector of a row that ends inside one is read element by element.
+// Rows wider than 16384 columns are walked in a loop (three passes, the later ones from L2).
+#include "common.h"
+#include "kernels.h"
+
+namespace {
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
+typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
+
+template <class T>
+struct Vec;  // E elements of T in 16 bytes
+template <>
+struct Vec<u16> {
+  static constexpr int E = 8;
+  static DV_DEVICE float get(u16 v) { return bf2f(v); }
+  static DV_DEVICE u16 put(float v) { return f2bf(v); }
+  static DV_DEVICE u32x4 load(const u16* p) { return *reinterpret_cast<const u32x4_a2*>(p); }
+  static DV_DEVICE void unpack(u32x4 r, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(r[i] << 16);
+      v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+    }
+  }
+  static DV_DEVICE void store(u16* p, const float (&v)[8]) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = pack2bf(v[2 * i], v[2 * i + 1]);
+    *reinterpret_cast<u32x4_a2*>(p) = r;
+  }
+};
+template <>
+struct Vec<float> {
+  static constexpr int E = 4;
+  static DV_DEVICE float get(float v) { return v; }
+  static DV_DEVICE float put(float v) { return v; }
+  static DV_DEVICE u32x4 load(const float* p) { return *reinterpret_cast<const u32x4_a4*>(p); }
+  static DV_DEVICE void unpack(u32x4 r, float (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
+  }
+  static DV_DEVICE void store(float* p, const float (&v)[4]) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __float_as_uint(v[i]);
+    *reinterpret_cast<u32x4_a4*>(p) = r;
+  }
+};
+
+// elements [c, c + E) of a row of D, zeros behind its end
+template <class T, int E = Vec<T>::E>
+DV_DEVICE void load_cols(const T* row, int c, int D, float (&v)[E]) {
+  if (c + E <= D) {
+    Vec<T>::unpack(Vec<T>::load(row + c), v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = c + e < D ? Vec<T>::get(row[c + e]) : 0.f;
+  }
+}
+template <class T, int E = Vec<T>::E>
+DV_DEVICE void store_cols(T* row, int c, int D, const float (&v)[E]) {
+  if (c + E <= D) {
+    Vec<T>::store(row + c, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (c + e < D) row[c + e] = Vec<T>::put(v[e]);
+  }
+}
+template <int E>
+DV_DEVICE void load_param(const float* w, int c, int D, float fill, float (&v)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = w && c + e < D ? w[c + e] : fill;
+}
+
+// sums of a and b over the LANES lanes of a row; LANES > 64 means the whole block
+template <int LANES>
+DV_DEVICE void row_sum2(float& a, float& b, float (*sh)[2]) {
+#pragma unroll
+  for (int o = (LANES < 64 ? LANES : 64) / 2; o > 0; o >>= 1) {
+    a += __shfl_xor(a, o, 64);
+    b += __shfl_xor(b, o, 64);
+  }
+  if constexpr (LANES > 64) {
+    __syncthreads();  // the previous use of sh is over
+    if ((threadIdx.x & 63) == 0) { sh[threadIdx.x >> 6][0] = a; sh[threadIdx.x >> 6][1] = b; }
+    __syncthreads();
+    a = b = 0.f;
+#pragma unroll
+    for (int i = 0; i < LANES / 64; ++i) { a += sh[i][0]; b += sh[i][1]; }
+  }
+}
+
+constexpr int block_of(int lanes) { return lanes > 256 ? lanes : 256; }
+
+template <class T, int LANES, int VECS>
+__global__ __launch_bounds__(block_of(LANES)) void ln_fwd_kernel(const T* __restrict__ x, int64_t ldx,
+                                                                 const float* __restrict__ w, const float* __restrict__ b,
+                                                                 T* __restrict__ y, float* __restrict__ stats, int64_t rows,
+                                                                 int D, float eps) {
+  constexpr int E = Vec<T>::E, RPB = block_of(LANES) / LANES;
+  __shared__ float sh[LANES > 64 ? LANES / 64 : 1][2];
+  const int lane = threadIdx.x % LANES;
+  float wv[VECS][E], bv[VECS][E];
+#pragma unroll
+  for (int k = 0; k < VECS; ++k) {
+    load_param<E>(w, (lane + k * LANES) * E, D, 1.f, wv[k]);
+    load_param<E>(b, (lane + k * LANES) * E, D, 0.f, bv[k]);
+  }
+  const float inv = 1.f / D;
+  for (int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / LANES; r < rows; r += (int64_t)gridDim.x * RPB) {
+    float v[VECS][E], s = 0.f, q = 0.f, none = 0.f;
+#pragma unroll
+    for (int k = 0; k < VECS; ++k) {
+      load_cols<T>(x + r * ldx, (lane + k * LANES) * E, D, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < VECS; ++k)
+#pragma unroll
+      for (int e = 0; e < E; ++e) s += v[k][e];
+    row_sum2<LANES>(s, none, sh);
+    const float mu = s * inv;
+#pragma unroll
+    for (int k = 0; k < VECS; ++k)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        v[k][e] = (lane + k * LANES) * E + e < D ? v[k][e] - mu : 0.f;
+        q += v[k][e] * v[k][e];
+      }
+    row_sum2<LANES>(q, none, sh);
+    const float rstd = 1.f / sqrtf(q * inv + eps);
+    if (lane == 0 && stats) { stats[2 * r] = mu; stats[2 * r + 1] = rstd; }
+#pragma unroll
+    for (int k = 0; k < VECS; ++k) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[k][e] = v[k][e] * rstd * wv[k][e] + bv[k][e];
+      store_cols<T>(y + r * D, (lane + k * LANES) * E, D, v[k]);
+    }
+  }
+}
+
+template <class T, int LANES, int VECS>
+__global__ __launch_bounds__(block_of(LANES)) void ln_bwd_kernel(const T* __restrict__ x, int64_t ldx,
+                                                                 const T* __restrict__ dy, int64_t ldg,
+                                                                 const float* __restrict__ w,
+                                                                 const float* __restrict__ stats, T* __restrict__ dx,
+                                                                 float* __restrict__ part, int64_t rows, int D) {
+  constexpr int E = Vec<T>::E, RPB = block_of(LANES) / LANES, COLS = LANES * VECS * E;
+  __shared__ float sh[LANES > 64 ? LANES / 64 : 1][2];
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  float wv[VECS][E], aw[VECS][E] = {}, ab[VECS][E] = {};
+#pragma unroll
+  for (int k = 0; k < VECS; ++k) load_param<E>(w, (lane + k * LANES) * E, D, 1.f, wv[k]);
+  const float inv = 1.f / D;
+  for (int64_t r = (int64_t)blockIdx.x * RPB + group; r < rows; r += (int64_t)gridDim.x * RPB) {
+    float v[VECS][E], g[VECS][E], s = 0.f, q = 0.f;
+#pragma unroll
+    for (int k = 0; k < VECS; ++k) {
+      load_cols<T>(x + r * ldx, (lane + k * LANES) * E, D, v[k]);
+      load_cols<T>(dy + r * ldg, (lane + k * LANES) * E, D, g[k]);
+    }
+    const float mu = stats[2 * r], rstd = stats[2 * r + 1];
+#pragma unroll
+    for (int k = 0; k < VECS; ++k)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {  // behind the row's end g is 0, so every sum there adds nothing
+        v[k][e] = (v[k][e] - mu) * rstd;
+        aw[k][e] += g[k][e] * v[k][e];
+        ab[k][e] += g[k][e];
+        g[k][e] *= wv[k][e];
+        s += g[k][e];
+        q += g[k][e] * v[k][e];
+      }
+    row_sum2<LANES>(s, q, sh);
+    s *= inv;
+    q *= inv;
+    if (dx) {
+#pragma unroll
+      for (int k = 0; k < VECS; ++k) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) g[k][e] = (g[k][e] - s - v[k][e] * q) * rstd;
+        store_cols<T>(dx + r * D, (lane + k * LANES) * E, D, g[k]);
+      }
+    }
+  }
+  if (!part) return;
+  part += (int64_t)blockIdx.x * 2 * D;
+  if constexpr (RPB == 1) {
+#pragma unroll
+    for (int k = 0; k < VECS; ++k)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int c = (lane + k * LANES) * E + e;
+        if (c < D) { part[c] = aw[k][e]; part[D + c] = ab[k][e]; }
+      }
+  } else {  // the block's row groups, added in order
+    __shared__ float fold[2][COLS];
+    for (int i = 0; i < RPB; ++i) {
+      if (group == i) {
+#pragma unroll
+        for (int k = 0; k < VECS; ++k)
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const int c = (lane + k * LANES) * E + e;
+            fold[0][c] = i ? fold[0][c] + aw[k][e] : aw[k][e];
+            fold[1][c] = i ? fold[1][c] + ab[k][e] : ab[k][e];
+          }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < D; c += block_of(LANES)) {
+      part[c] = fold[0][c];
+      part[D + c] = fold[1][c];
+    }
+  }
+}
+
+// Rows of any width: one block a row, the row read three times (twice from cache).
+template <class T>
+__global__ __launch_bounds__(1024) void ln_fwd_wide_kernel(const T* __restrict__ x, int64_t ldx, const float* __restrict__ w,
+                                                           const float* __restrict__ b, T* __restrict__ y,
+                                                           float* __restrict__ stats, int D, float eps) {
+  __shared__ float sh[16][2];
+  const int64_t r = blockIdx.x;
+  const T* row = x + r * ldx;
+  float s = 0.f, q = 0.f, none = 0.f;
+  for (int c = threadIdx.x; c < D; c += 1024) s += Vec<T>::get(row[c]);
+  row_sum2<1024>(s, none, sh);
+  const float mu = s / D;
+  for (int c = threadIdx.x; c < D; c += 1024) {
+    const float d = Vec<T>::get(row[c]) - mu;
+    q += d * d;
+  }
+  row_sum2<1024>(q, none, sh);
+  const float rstd = 1.f / sqrtf(q / D + eps);
+  if (threadIdx.x == 0 && stats) { stats[2 * r] = mu; stats[2 * r + 1] = rstd; }
+  for (int c = threadIdx.x; c < D; c += 1024)
+    y[r * D + c] = Vec<T>::put((Vec<T>::get(row[c]) - mu) * rstd * (w ? w[c] : 1.f) + (b ? b[c] : 0.f));
+}
+
+template <class T>
+__global__ __launch_bounds__(1024) void ln_bwd_wide_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ dy,
+                                                           int64_t ldg, const float* __restrict__ w,
+                                                           const float* __restrict__ stats, T* __restrict__ dx, int D) {
+  __shared__ float sh[16][2];
+  const int64_t r = blockIdx.x;
+  const float mu = stats[2 * r], rstd = stats[2 * r + 1];
+  float s = 0.f, q = 0.f;
+  for (int c = threadIdx.x; c < D; c += 1024) {
+    const float h = Vec<T>::get(dy[r * ldg + c]) * (w ? w[c] : 1.f);
+    s += h;
+    q += h * (Vec<T>::get(x[r * ldx + c]) - mu) * rstd;
+  }
+  row_sum2<1024>(s, q, sh);
+  s /= D;
+  q /= D;
+  for (int c = threadIdx.x; c < D; c += 1024) {
+    const float h = Vec<T>::get(dy[r * ldg + c]) * (w ? w[c] : 1.f);
+    dx[r * D + c] = Vec<T>::put((h - s - (Vec<T>::get(x[r * ldx + c]) - mu) * rstd * q) * rstd);
+  }
+}
+// its parameter gradients: a thread a column, blockIdx.y a strip of rows
+template <class T>
+__global__ __launch_bounds__(256) void ln_param_wide_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ dy,
+                                                            int64_t ldg, const float* __restrict__ stats,
+                                                            float* __restrict__ part, int64_t rows, int D) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= D) return;
+  const int64_t r0 = rows * blockIdx.y / gridDim.y, r1 = rows * (blockIdx.y + 1) / gridDim.y;
+  float aw = 0.f, ab = 0.f;
+  for (int64_t r = r0; r < r1; ++r) {
+    const float g = Vec<T>::get(dy[r * ldg + c]);
+    aw += g * (Vec<T>::get(x[r * ldx + c]) - stats[2 * r]) * stats[2 * r + 1];
+    ab += g;
+  }
+  part[(int64_t)blockIdx.y * 2 * D + c] = aw;
+  part[(int64_t)blockIdx.y * 2 * D + D + c] = ab;
+}
+
+// dw / db [D] (+)= sum over the slab's rows: 16 columns a block, 16 row lanes a column
+__global__ __launch_bounds__(256) void ln_fold_kernel(const float* __restrict__ part, int parts, int D,
+                                                      float* __restrict__ dw, float* __restrict__ db, int acc_w, int acc_b) {
+  __shared__ float sh[16][17];
+  const int j = threadIdx.x & 15, i = threadIdx.x >> 4;
+  const int64_t c = (int64_t)blockIdx.x * 16 + j;
+  float s = 0.f;
+  if (c < 2 * (int64_t)D)
+    for (int p = i; p < parts; p += 16) s += part[(int64_t)p * 2 * D + c];
+  sh[i][j] = s;
+  __syncthreads();
+  if (i == 0 && c < 2 * (int64_t)D) {
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t += sh[k][j];
+    float* out = c < D ? dw : db;
+    const int64_t o = c < D ? c : c - D;
+    if (out) out[o] = (c < D ? acc_w : acc_b) ? out[o] + t : t;
+  }
+}
+
+constexpr int MAX_ELEMS = 32;  // fp32 values of a row a lane holds
+
+// f(LANES, VECS) of the narrowest form that holds D columns: the fewest lanes with at most
+// MAX_ELEMS values each, so that narrow rows share a wave
+template <class T, class F>
+bool with_form(int D, F&& f) {
+  constexpr int E = Vec<T>::E, V = MAX_ELEMS / E;
+  const int vecs = (D + E - 1) / E;
+#define LN_FORM(L, K) \
+  if (vecs <= (L) * (K)) { f(std::integral_constant<int, L>{}, std::integral_constant<int, K>{}); return true; }
+  LN_FORM(16, 1)
+  LN_FORM(32, 1)
+  LN_FORM(64, 1)
+  LN_FORM(64, 2)
+  LN_FORM(64, 4)
+  if constexpr (V > 4) { LN_FORM(64, V) }
+  LN_FORM(256, 2)
+  LN_FORM(256, 4)
+  if constexpr (V > 4) { LN_FORM(256, V) }
+  LN_FORM(512, V)
+#undef LN_FORM
+  return false;
+}
+
+template <class T>
+void ln_fwd(const T* x, int64_t ldx, const float* w, const float* b, T* y, float* stats, int64_t rows, int D, float eps,
+            hipStream_t st) {
+  const bool held = with_form<T>(D, [&](auto l, auto k) {
+    constexpr int L = decltype(l)::value, K = decltype(k)::value, RPB = block_of(L) / L;
+    const int64_t grid = std::min<int64_t>((rows + RPB - 1) / RPB, 256 * 8);
+    ln_fwd_kernel<T, L, K><<<(unsigned)grid, block_of(L), 0, st>>>(x, ldx, w, b, y, stats, rows, D, eps);
+  });
+  if (!held) ln_fwd_wide_kernel<T><<<(unsigned)rows, 1024, 0, st>>>(x, ldx, w, b, y, stats, D, eps);
+}
+
+template <class T>
+int ln_bwd(const T* x, int64_t ldx, const T* dy, int64_t ldg, const float* w, const float* stats, T* dx, float* part,
+           int parts, int64_t rows, int D, hipStream_t st) {
+  const bool held = with_form<T>(D, [&](auto l, auto k) {
+    constexpr int L = decltype(l)::value, K = decltype(k)::value;
+    ln_bwd_kernel<T, L, K><<<(unsigned)parts, block_of(L), 0, st>>>(x, ldx, dy, ldg, w, stats, dx, part, rows, D);
+  });
+  if (!held) {
+    if (dx) ln_bwd_wide_kernel<T><<<(unsigned)rows, 1024, 0, st>>>(x, ldx, dy, ldg, w, stats, dx, D);
+    if (part) {
+      const dim3 grid((unsigned)((D + 255) / 256), (unsigned)parts);
+      ln_param_wide_kernel<T><<<grid, 256, 0, st>>>(x, ldx, dy, ldg, stats, part, rows, D);
+    }
+  }
+  return 0;
+}
+}  // namespace
+
+int dv_layer_norm_parts(int is_bf16, int64_t rows, int D) {
+  int per = 0;
+  auto rpb = [&](auto l, auto) { per = block_of(decltype(l)::value) / decltype(l)::value; };
+  const bool held = is_bf16 ? with_form<u16>(D, rpb) : with_form<float>(D, rpb);
+  if (!held) return (int)std::min<int64_t>(rows, 64);
+  return (int)std::min<int64_t>((rows + per - 1) / per, 512);
+}
+
+int dv_layer_norm_fwd(const void* x, int is_bf16, int64_t ldx, const float* w, const float* b, void* y, float* stats,
+                      int64_t rows, int D, float eps, hipStream_t st) {
+  if (rows <= 0 || rows > 0x7fffffff || D <= 0 || ldx < D) return -1;
+  if (is_bf16) ln_fwd<u16>((const u16*)x, ldx, w, b, (u16*)y, stats, rows, D, eps, st);
+  else ln_fwd<float>((const float*)x, ldx, w, b, (float*)y, stats, rows, D, eps, st);
+  return 0;
+}
+
+int dv_layer_norm_bwd(const void* x, int is_bf16, int64_t ldx, const void* dy, int64_t ldg, const float* w,
+                      const float* stats, void* dx, float* part, int parts, float* dw, float* db, int acc_w, int acc_b,
+                      int64_t rows, int D, hipStream_t st) {
+  if (rows <= 0 || rows > 0x7fffffff || D <= 0 || ldx < D || ldg < D || parts <= 0 ||
+      parts != dv_layer_norm_parts(is_bf16, rows, D) || (!part && (dw || db)))
+    return -1;
+  if (is_bf16) ln_bwd<u16>((const u16*)x, ldx, (const u16*)dy, ldg, w, stats, (u16*)dx, part, parts, rows, D, st);
+  else ln_bwd<float>((const float*)x, ldx, (const float*)dy, ldg, w, stats, (float*)dx, part, parts, rows, D, st);
+  if (dw || db) {
+    const unsigned grid = (unsigned)((2 * (int64_t)D + 15) / 16);
+    ln_fold_kernel<<<grid, 256, 0, st>>>(part, parts, D, dw, db, acc_w, acc_b);
+  }
+  return 0;
+}

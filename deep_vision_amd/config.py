@@ -26,7 +26,7 @@ class TrainConfig:
     model: str                      # deep_vision_amd.models.MODELS key
     batch_size: int                 # global (batch_semantics == "global") or per replica
     total_epochs: int
-    optimizer: str                  # "sgd" | "adam" | "rmsprop"
+    optimizer: str                  # "sgd" | "adam" | "adamw" | "rmsprop"
     optimizer_params: Dict[str, Any]
     scheduler: Optional[str] = None  # "plateau" | "step" | "lambda" | "manual_plateau" | "linear_decay" | None
     scheduler_params: Dict[str, Any] = field(default_factory=dict)

@@ -16,7 +16,7 @@ from ..ops.common import native, unsupported
 
 __all__ = [
     "Conv2d", "ConvTranspose2d", "Linear", "BatchNorm2d", "ReLU", "LeakyReLU", "Tanh", "Sigmoid", "MaxPool2d",
-    "AvgPool2d", "AdaptiveAvgPool2d", "Dropout", "Upsample", "LocalResponseNorm", "Flatten", "Sequential",
+    "AvgPool2d", "AdaptiveAvgPool2d", "Dropout", "Upsample", "LocalResponseNorm", "LayerNorm", "Flatten", "Sequential",
     "ZeroPad2d", "ReflectionPad2d", "ChannelShuffle", "Identity", "FusedSequential",
 ]
 
@@ -188,6 +188,14 @@ class LocalResponseNorm(tnn.LocalResponseNorm):
         from ..ops.lrn import local_response_norm
 
         return local_response_norm(x, self.size, self.alpha, self.beta, self.k)
+
+
+class LayerNorm(tnn.LayerNorm):
+    """torch.nn.LayerNorm: statistics over the last dimensions of each row (ops.layer_norm). For a
+    channels-last feature map normalise ``x.permute(0, 2, 3, 1)``: its rows are read in place."""
+
+    def forward(self, x):
+        return F.layer_norm(x, self.normalized_shape, self.weight, self.bias, self.eps)
 
 
 class ZeroPad2d(tnn.ZeroPad2d):

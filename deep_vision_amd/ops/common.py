@@ -10,6 +10,7 @@ GPU tensor conventions (all native ops):
 from __future__ import annotations
 
 import os
+import weakref
 
 import torch
 
@@ -177,6 +178,68 @@ def grad_sink(param):
     if torch.is_grad_enabled():  # double-backward: keep autograd semantics
         return None
     return g
+
+
+def accumulation_sink(ctx, index, param):
+    """``grad_sink(param)`` where this backward pass is going to add the gradient of input ``index``
+    to ``param.grad``; None under ``torch.autograd.grad`` (which wants the gradient returned and
+    ``.grad`` untouched), for a pass that leaves the parameter out, and where the parameter has
+    hooks that read its gradient."""
+    sink = grad_sink(param)
+    if sink is None or param._backward_hooks:
+        return None
+    try:
+        return sink if torch._C._will_engine_execute_node(ctx.next_functions[index][0]) else None
+    except RuntimeError:  # the engine's answer for a leaf that torch.autograd.grad captures
+        return None
+
+
+_GRAPHS = {}  # id(leaf) -> [(weak reference to an autograd node that uses it, the node's stream)]
+
+
+def track_leaves(ctx, *leaves):
+    """Remember which stream the live graphs of ``leaves`` were built on, and refuse to capture a new
+    one while an older lives: the leaf's gradient accumulation belongs to the older graph's stream,
+    and a captured backward pass that joins a stream outside the capture ends the process."""
+    stream = stream_handle()
+    capturing = torch.cuda.is_current_stream_capturing()
+    me = weakref.ref(ctx)
+    for t in leaves:
+        if t is None or not t.requires_grad or not t.is_leaf:
+            continue
+        alive = [e for e in _GRAPHS.get(id(t), ()) if e[0]() is not None]
+        if capturing and any(s != stream for _, s in alive):
+            raise RuntimeError("an eager autograd graph of this tensor is still alive (a loss or output that holds it): "
+                               "delete it before capturing a backward pass over the same tensor")
+        alive.append((me, stream))
+        _GRAPHS[id(t)] = alive
+    if len(_GRAPHS) > 4096:
+        for k in [k for k, v in _GRAPHS.items() if all(e[0]() is None for e in v)]:
+            del _GRAPHS[k]
+
+
+def same_device(what, x, *others):
+    """Every tensor of ``others`` (None allowed) lives where ``x`` does."""
+    for t in others:
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{what}: all tensors must be on {x.device}, got one on {t.device}")
+
+
+class on_device:
+    """Launch on the tensor's own device: the kernels run on the current stream of ``x``'s device
+    whichever device is current. Free where that is the current one already."""
+
+    def __init__(self, x):
+        i = x.device.index
+        self.guard = None if i is None or i == torch.cuda.current_device() else torch.cuda.device(i)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
 def workspace(owner, key, shape, device, dtype=F32):

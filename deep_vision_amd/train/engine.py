@@ -26,9 +26,9 @@ from ..parallel.ddp import DataParallel
 from ..parallel.watchdog import CommWatchdog, install_backend_error_handling
 from ..profiling import StepTimer
 from ..utils.fault import FaultInjector, NonFiniteGuard, Watchdog
-from .optim import FusedAdam, FusedRMSprop, FusedSGD
+from .optim import FusedAdam, FusedAdamW, FusedRMSprop, FusedSGD
 
-OPTIMIZERS = {"sgd": FusedSGD, "adam": FusedAdam, "rmsprop": FusedRMSprop}
+OPTIMIZERS = {"sgd": FusedSGD, "adam": FusedAdam, "adamw": FusedAdamW, "rmsprop": FusedRMSprop}
 
 
 def seed_everything(seed: int, rank: int = 0):

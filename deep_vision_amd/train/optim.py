@@ -5,7 +5,7 @@ views into it) and their ``.grad``s are views into a matching flat gradient buff
 launch (csrc/loss_optim.hip) updates the whole model per step, and the data-parallel layer
 all-reduces slices of the same flat gradient buffer in place (no bucket copies).
 
-Update rules match torch.optim.SGD / Adam / RMSprop exactly (same state names, same
+Update rules match torch.optim.SGD / Adam / AdamW / RMSprop exactly (same state names, same
 ``state_dict`` format), as used by the reference configs (R/ResNet/pytorch/train.py:26-215:
 SGD momentum .9 + wd, RMSprop for MobileNet; Adam for LeNet/YOLO/Hourglass/GANs).
 On CPU the same classes run the identical math with torch ops.
@@ -13,10 +13,12 @@ On CPU the same classes run the identical math with torch ops.
 from __future__ import annotations
 
 import math
+from bisect import bisect_left
 
 import torch
 
 from .._ext import lib, ptr, stream_handle
+from ..ops.common import on_device
 
 
 class _FlatOptimizer(torch.optim.Optimizer):
@@ -99,17 +101,34 @@ class _FlatOptimizer(torch.optim.Optimizer):
                 p._dv_flat = shared
             for p, (off, _) in zip(ps, offs):
                 p._dv_off = off
-        states = {name: torch.zeros(total, dtype=torch.float32, device=dev) for name in self.STATE_NAMES}
-        f = dict(param=pflat, grad=gflat, views=views, gviews=gviews, offsets=offs, states=states, step=0,
-                 first=True, shared=shared)
+        f = dict(param=pflat, grad=gflat, views=views, gviews=gviews, offsets=offs, step=0, first=True, shared=shared)
+        f["states"] = self._new_states(f)
         if old is not None:  # re-bound after the parameters moved: carry the optimizer state over
             f["step"], f["first"] = old["step"], old["first"]
             if old.get("hp") is not None:
                 f["hp"] = old["hp"]
-            for (o_off, n), (n_off, _) in zip(old["offsets"], offs):
-                for name in self.STATE_NAMES:
-                    f["states"][name][n_off:n_off + n].copy_(old["states"][name][o_off:o_off + n])
+            self._carry_states(old, f)
         return f
+
+    # ---------------- the optimizer's state: fp32 buffers laid out as the flat parameters ----------------
+    def _new_states(self, f):
+        return {name: torch.zeros_like(f["param"]) for name in self.STATE_NAMES}
+
+    def _carry_states(self, old, f):
+        for (o_off, n), (n_off, _) in zip(old["offsets"], f["offsets"]):
+            for name in self.STATE_NAMES:
+                f["states"][name][n_off:n_off + n].copy_(old["states"][name][o_off:o_off + n])
+
+    def _save_state(self, f, i, shape):
+        """State-dict entries of the group's ``i``-th parameter."""
+        off, n = f["offsets"][i]
+        return {name: buf[off:off + n].view(shape).clone() for name, buf in f["states"].items()}
+
+    def _load_state(self, f, i, st):
+        off, n = f["offsets"][i]
+        for name in self.STATE_NAMES:
+            if name in st:
+                f["states"][name][off:off + n].copy_(st[name].reshape(-1).to(f["param"].device))
 
     def _check_binding(self):
         """Each parameter must still be a view of THIS optimizer's flat buffer. When a later
@@ -218,6 +237,14 @@ class _FlatOptimizer(torch.optim.Optimizer):
     def flat_grads(self):
         return [f["grad"] for f in self._flat if f]
 
+    def flat_params(self):
+        """Each group's parameters as the one flat fp32 buffer the update runs over."""
+        return [f["param"] for f in self._flat if f]
+
+    def flat_states(self):
+        """Each group's live state buffers by name (``FusedAdamW`` documents its 8-bit ones)."""
+        return [dict(f["states"]) for f in self._flat if f]
+
     @torch.no_grad()
     def zero_grad(self, set_to_none: bool = False):
         self._check_binding()
@@ -306,10 +333,8 @@ class _FlatOptimizer(torch.optim.Optimizer):
         for group, f in zip(self.param_groups, self._flat):
             if f is None:
                 continue
-            for (off, n), p in zip(f["offsets"], group["params"]):
-                st = {}
-                for name, buf in f["states"].items():
-                    st[name] = buf[off:off + n].view(p.shape).clone()
+            for i, p in enumerate(group["params"]):
+                st = self._save_state(f, i, p.shape)
                 if self.STATE_NAMES and not f["first"]:
                     st["step"] = torch.tensor(float(f["step"]))
                     state[idx] = st
@@ -340,13 +365,11 @@ class _FlatOptimizer(torch.optim.Optimizer):
                 continue
             f["step"] = int(sg.get("_dv_step", 0))
             any_state = False
-            for (off, n), p in zip(f["offsets"], group["params"]):
+            for i in range(len(group["params"])):
                 st = state_dict["state"].get(idx, state_dict["state"].get(str(idx)))
                 if st:
                     any_state = True
-                    for name in self.STATE_NAMES:
-                        if name in st:
-                            f["states"][name][off:off + n].copy_(st[name].reshape(-1).to(f["param"].device))
+                    self._load_state(f, i, st)
                     if "step" in st and f["step"] == 0:
                         f["step"] = int(float(st["step"]))
                 idx += 1
@@ -418,6 +441,172 @@ class FusedAdam(_FlatOptimizer):
         p.addcdiv_(m, denom, value=-g["lr"] / bc1)
 
 
+def _mix(h):
+    """csrc/adamw.hip mix(): 32 mixed bits of a whole number below 2^32, held in int64."""
+    h = h ^ (h >> 16)
+    h = (h * 0x6C8E9CF5) & 0xFFFFFFFF
+    h = h ^ (h >> 15)
+    h = (h * 0x5D2A4B35) & 0xFFFFFFFF
+    return h ^ (h >> 16)
+
+
+class FusedAdamW(_FlatOptimizer):
+    """AdamW (decoupled weight decay, torch.optim.AdamW's update) over the flat buffer, one launch a
+    group (csrc/adamw.hip). ``state_bits=32`` keeps fp32 moments ``exp_avg`` / ``exp_avg_sq``.
+
+    ``state_bits=8`` keeps a quarter of that: ``exp_avg`` and ``exp_avg_root`` (the square root of the
+    second moment) as ``torch.float8_e4m3fn`` codes, each block of 256 values of a tensor times an
+    fp32 scale (``*_scale``). A tensor's codes start at a block of their own and are padded with
+    zeros to whole blocks, in the order of the group's parameters. Codes are rounded
+    stochastically from a hash of (``seed``, step, place): a run repeats bit for bit. Both kinds of
+    state load from either kind of checkpoint."""
+
+    STATE_NAMES = ("exp_avg", "exp_avg_sq")
+    BLOCK, CHUNK = 256, 4096  # csrc/kernels.h DV_ADAMW_BLOCK, DV_ADAMW_CHUNK
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"FusedAdamW: state_bits must be 8 or 32, got {state_bits!r}")
+        if not (0 <= betas[0] < 1 and 0 <= betas[1] < 1):
+            raise ValueError(f"FusedAdamW: betas must lie in [0, 1), got {betas!r}")
+        if eps < 0 or lr < 0 or weight_decay < 0:
+            raise ValueError(f"FusedAdamW: lr, eps and weight_decay must not be negative, got {lr!r}, {eps!r}, {weight_decay!r}")
+        self.state_bits, self.seed = state_bits, int(seed) & 0xFFFFFFFF
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def _hparams(self, group, step):
+        b1, b2 = group["betas"]
+        return float(group["lr"]), 1 - b1 ** step, 1 - b2 ** step
+
+    # ---------------- 8-bit state ----------------
+    def _new_states(self, f):
+        if self.state_bits == 32:
+            return super()._new_states(f)
+        dev, block, chunks, f["blocks"] = f["param"].device, 0, [], []
+        for off, n in f["offsets"]:
+            e = -(-n // self.BLOCK)
+            f["blocks"].append((block, e))
+            chunks += [(off + k, block + k // self.BLOCK, min(self.CHUNK, n - k)) for k in range(0, n, self.CHUNK)]
+            block += e
+        chunks.sort()  # by place in the flat buffer: a run of whole tensors there is a run of chunks
+        f["chunk_starts"] = [c[0] for c in chunks]
+        f["chunks"] = torch.tensor(chunks, dtype=torch.int64).reshape(-1, 3).to(dev)
+        out = {}
+        for name in ("exp_avg", "exp_avg_root"):
+            out[name] = torch.zeros(block * self.BLOCK, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+            out[name + "_scale"] = torch.zeros(block, dtype=torch.float32, device=dev)
+        return out
+
+    def _slices(self, f, i):
+        """The group's ``i``-th parameter's part of each 8-bit state buffer."""
+        b, e = f["blocks"][i]
+        return {name: buf[b:b + e] if name.endswith("_scale") else buf[b * self.BLOCK:(b + e) * self.BLOCK]
+                for name, buf in f["states"].items()}
+
+    def _carry_states(self, old, f):
+        if self.state_bits == 32:
+            return super()._carry_states(old, f)
+        for name, buf in f["states"].items():
+            buf.view(torch.uint8).copy_(old["states"][name].view(torch.uint8))
+
+    def _save_state(self, f, i, shape):
+        if self.state_bits == 32:
+            return super()._save_state(f, i, shape)
+        return {name: t.clone() for name, t in self._slices(f, i).items()}
+
+    def _load_state(self, f, i, st):
+        n = f["offsets"][i][1]
+        packed = "exp_avg_root" in st
+        if self.state_bits == 32 and packed:
+            wide = {k: (st[k].float().view(-1, self.BLOCK) * st[k + "_scale"].float()[:, None]).view(-1)[:n]
+                    for k in ("exp_avg", "exp_avg_root")}
+            st = {"exp_avg": wide["exp_avg"], "exp_avg_sq": wide["exp_avg_root"] ** 2}
+        if self.state_bits == 32:
+            return super()._load_state(f, i, st)
+        mine = self._slices(f, i)
+        for name in ("exp_avg", "exp_avg_root"):
+            if packed:
+                for k in (name, name + "_scale"):
+                    if st[k].numel() != mine[k].numel():
+                        raise ValueError(f"FusedAdamW: {k} of a saved 8-bit state has {st[k].numel()} entries, "
+                                         f"expected {mine[k].numel()}")
+                mine[name].view(torch.uint8).copy_(st[name].contiguous().view(torch.uint8))
+                mine[name + "_scale"].copy_(st[name + "_scale"])
+            elif "exp_avg" in st and "exp_avg_sq" in st:  # 32-bit moments: rounded to nearest, once
+                t = st["exp_avg"] if name == "exp_avg" else st["exp_avg_sq"].sqrt()
+                wide = torch.zeros(mine[name].numel(), dtype=torch.float32, device=mine[name].device)
+                wide[:n].copy_(t.reshape(-1))
+                self._store8(mine, name, wide.view(-1, self.BLOCK), 0x80000)
+
+    def _store8(self, states, name, t, noise):
+        """Blocks ``t`` [blocks][256] as codes and scales, the kernel's arithmetic (csrc/adamw.hip)."""
+        if not t.numel():
+            return
+        top = t.abs().amax(1, keepdim=True)
+        up = torch.where(top >= 2.0 ** -100, torch.full_like(top, 448.0) / top, torch.zeros_like(top))
+        s = t.abs() * up
+        code = (((s * 2.0 ** -120).view(torch.int32).long() + noise) >> 20).clamp_(max=126)
+        code = torch.where(s < 1e30, code, 127)
+        if name == "exp_avg":
+            code = code + 128 * (t < 0)
+        else:
+            code = torch.maximum(code, (t > 0).long())
+        states[name].view(torch.uint8).copy_(code.to(torch.uint8).view(-1))
+        states[name + "_scale"].copy_((top * torch.full_like(top, 1 / 448.0))[:, 0])
+
+    # ---------------- update ----------------
+    def _update(self, g, f, off, n, gs):
+        if not n:
+            return
+        b1, b2 = g["betas"]
+        _, bc1, bc2 = self._hparams(g, f["step"])
+        p, gr, s = f["param"][off:off + n], f["grad"][off:off + n], f["states"]
+        if p.is_cuda:
+            args = (float(g["lr"]), float(b1), float(b2), float(g["eps"]), float(g["weight_decay"]), float(bc1), float(bc2),
+                    float(gs))
+            with on_device(p):
+                if self.state_bits == 32:
+                    lib().adamw32(ptr(p), ptr(gr), ptr(s["exp_avg"][off:off + n]), ptr(s["exp_avg_sq"][off:off + n]), n,
+                                  *args, self._hp_ptr(f), self._skip_ptr(), stream_handle())
+                    return
+                lo, hi = bisect_left(f["chunk_starts"], off), bisect_left(f["chunk_starts"], off + n)
+                lib().adamw8(ptr(f["param"]), ptr(f["grad"]), ptr(s["exp_avg"]), ptr(s["exp_avg_scale"]),
+                             ptr(s["exp_avg_root"]), ptr(s["exp_avg_root_scale"]), ptr(f["chunks"][lo:hi]), hi - lo, *args,
+                             f["step"] & 0xFFFFFFFF, self.seed, self._hp_ptr(f), self._skip_ptr(), stream_handle())
+            return
+        if self.state_bits == 32:
+            self._update_cpu(g, p, gr * gs, s["exp_avg"][off:off + n], s["exp_avg_sq"][off:off + n], bc1, bc2)
+            return
+        for i, (o, k) in enumerate(f["offsets"]):
+            if k and off <= o < off + n:
+                self._update8_cpu(g, f, i, gs, bc1, bc2)
+
+    @staticmethod
+    def _update_cpu(g, p, grad, m, v, bc1, bc2):
+        b1, b2 = g["betas"]
+        m.copy_(m * b1 + grad * (1 - b1))
+        v.copy_(v * b2 + (grad * grad) * (1 - b2))
+        p.copy_(p * (1 - g["lr"] * g["weight_decay"]) - g["lr"] / bc1 * (m / (v.sqrt() / math.sqrt(bc2) + g["eps"])))
+
+    def _update8_cpu(self, g, f, i, gs, bc1, bc2):
+        (o, n), (block, e), mine = f["offsets"][i], f["blocks"][i], self._slices(f, i)
+        dev = f["param"].device
+        grad = torch.zeros(e * self.BLOCK, device=dev)
+        grad[:n] = f["grad"][o:o + n] * gs
+        m, r = ((mine[k].float().view(e, self.BLOCK) * mine[k + "_scale"][:, None]).view(-1)
+                for k in ("exp_avg", "exp_avg_root"))
+        v, p = r * r, torch.zeros_like(grad)
+        p[:n] = f["param"][o:o + n]
+        self._update_cpu(g, p, grad, m, v, bc1, bc2)
+        f["param"][o:o + n] = p[:n]
+        key = _mix((self.seed + f["step"] * 0x9E3779B1) & 0xFFFFFFFF)
+        place = torch.arange(block * self.BLOCK, (block + e) * self.BLOCK, device=dev)
+        noise = _mix(((place & 0xFFFFFFFF) * 0x2545F491 + (place >> 32) * 0x7A6B3C5D + key) & 0xFFFFFFFF).view(e, self.BLOCK)
+        self._store8(mine, "exp_avg", m.view(e, self.BLOCK), noise & 0xFFFFF)
+        # the host's vector square root may be an ulp off: through 64 bits it is the kernel's
+        self._store8(mine, "exp_avg_root", v.double().sqrt().float().view(e, self.BLOCK), noise >> 12)
+
+
 class FusedRMSprop(_FlatOptimizer):
     STATE_NAMES = ("square_avg", "momentum_buffer", "grad_avg")
 
@@ -450,4 +639,4 @@ class FusedRMSprop(_FlatOptimizer):
             p.addcdiv_(grad, avg, value=-g["lr"])
 
 
-OPTIMIZERS = {"SGD": FusedSGD, "Adam": FusedAdam, "RMSprop": FusedRMSprop}
+OPTIMIZERS = {"SGD": FusedSGD, "Adam": FusedAdam, "AdamW": FusedAdamW, "RMSprop": FusedRMSprop}
