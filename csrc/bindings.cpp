@@ -361,6 +361,34 @@ PYBIND11_MODULE(_C, m) {
       throw std::runtime_error("adamw8: no chunks");
     check_last("adamw8");
   });
+  // shared arguments of linear_xent: (x, ldx, w, ldw, bias, labels, N, V, D, width, ignore, smooth, reduction)
+#define XENT_ARGS uptr x, int64_t ldx, uptr w, int64_t ldw, uptr bias, uptr labels, int N, int V, int D, int width, int64_t ignore, float smooth, int reduction
+#define XENT(go, total) \
+  DvXent{reinterpret_cast<const uint16_t*>(x), reinterpret_cast<const uint16_t*>(w), ldx, ldw, CFP(bias), \
+         reinterpret_cast<const int64_t*>(labels), N, V, D, width, ignore, smooth, reduction, CFP(go), CFP(total)}
+  m.def("linear_xent_fwd_bytes", [](XENT_ARGS) { return dv_linear_xent_fwd_bytes(XENT(0, 0)); });
+  m.def("linear_xent_fwd", [](XENT_ARGS, uptr ws, uptr lse, uptr rows, uptr total, uptr out, uptr st) {
+    if (dv_linear_xent_fwd(XENT(0, 0), P(ws), FP(lse), FP(rows), FP(total), FP(out), ST(st)))
+      throw std::runtime_error("linear_xent_fwd: unsupported shape");
+    check_last("linear_xent_fwd");
+  });
+  m.def("linear_xent_bwd_bytes", [](XENT_ARGS, int need_x, int need_w, int need_b, int have_wt) {
+    return dv_linear_xent_bwd_bytes(XENT(0, 0), need_x, need_w, need_b, have_wt);
+  });
+  m.def("linear_xent_bwd", [](XENT_ARGS, uptr go, uptr total, uptr ws, uptr lse, uptr wt, int64_t ldwt, uptr dx, uptr dw,
+                              int dw_f32, int dw_add, uptr db, int db_add, uptr st) {
+    if (dv_linear_xent_bwd(XENT(go, total), P(ws), CFP(lse), CP(wt), ldwt, P(dx), P(dw), dw_f32, dw_add, FP(db), db_add,
+                           ST(st)))
+      throw std::runtime_error("linear_xent_bwd: unsupported shape");
+    check_last("linear_xent_bwd");
+  });
+#undef XENT
+#undef XENT_ARGS
+  m.attr("XENT_MAX_ROWS") = DV_XENT_MAX_ROWS;
+  m.def("pack_rows", [](uptr src, int bf16, int64_t lds, int64_t rows, int cols, uptr dst, int64_t ldd, uptr st) {
+    if (dv_pack_rows(CP(src), bf16, lds, rows, cols, P(dst), ldd, ST(st))) throw std::runtime_error("pack_rows: unsupported shape");
+    check_last("pack_rows");
+  });
   m.attr("ADAMW_BLOCK") = DV_ADAMW_BLOCK;
   m.attr("ADAMW_CHUNK") = DV_ADAMW_CHUNK;
   m.def("layer_norm_parts", [](int bf16, int64_t rows, int D) { return dv_layer_norm_parts(bf16, rows, D); });

@@ -258,6 +258,32 @@ int dv_adamw32(const DvAdamW& a, float* p, const float* g, float* m, float* v, i
 int dv_adamw8(const DvAdamW& a, const void* chunks, int nchunks, float* p, const float* g, uint8_t* m8, float* ms,
               uint8_t* r8, float* rs, hipStream_t st);
 
+// ---- linear + softmax cross entropy (linear_xent.hip) ----
+enum { DV_XENT_NONE = 0, DV_XENT_MEAN = 1, DV_XENT_SUM = 2 };
+constexpr int DV_XENT_MAX_ROWS = 1 << 22;
+struct DvXent {
+  const uint16_t *x, *w;   // bf16 [N][ldx], [V][ldw]: D columns, zeros from `width` on
+  int64_t ldx, ldw;
+  const float* bias;       // [V] or null
+  const int64_t* labels;   // [N]
+  int N, V, D, width;      // D: width rounded up to 64
+  int64_t ignore;          // label of the rows that take no part (as do labels outside [0, V))
+  float smooth;
+  int reduction;
+  const float* go;         // backward: the upstream gradient, [N] for DV_XENT_NONE, else [1]
+  const float* total;      // backward, mean: [1] is the number of rows that count
+};
+int64_t dv_linear_xent_fwd_bytes(const DvXent& a);
+int64_t dv_linear_xent_bwd_bytes(const DvXent& a, int need_x, int need_w, int need_b, int have_wt);
+// lse [N] and loss_rows [N] may be null; out (the reduced loss) and total [2] go together, null for DV_XENT_NONE
+int dv_linear_xent_fwd(const DvXent& a, void* ws, float* lse, float* loss_rows, float* total, float* out, hipStream_t st);
+// dx [N][width] bf16, dw [V][width] bf16 or fp32 (added to where dw_add), db [V]; each may be null.
+// wt: bf16 [width][ldwt] = w transposed, zeros behind V, or null
+int dv_linear_xent_bwd(const DvXent& a, void* ws, const float* lse, const void* wt, int64_t ldwt, void* dx, void* dw,
+                       int dw_f32, int dw_add, float* db, int db_add, hipStream_t st);
+// bf16 [rows][ldd] = src [rows][cols] (row stride lds), zeros behind cols
+int dv_pack_rows(const void* src, int is_bf16, int64_t lds, int64_t rows, int cols, void* dst, int64_t ldd, hipStream_t st);
+
 // ---- layer norm (layer_norm.hip) ----
 // x / dy rows at strides ldx / ldg, y / dx dense; stats [rows][2] = mean, rstd; w / b / dw / db may be null.
 // part: [parts][2][D] scratch with parts = dv_layer_norm_parts(); acc_w / acc_b add into dw / db.

@@ -8,7 +8,8 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as TF
 
-from .common import BF16, F32, lib, native, ptr, stream_handle
+from .common import (BF16, F32, accumulation_sink, lib, native, on_device, ptr, same_device, stream_handle,
+                     track_leaves)
 
 
 class _XentFn(torch.autograd.Function):
@@ -46,6 +47,168 @@ def cross_entropy(logits, labels, label_smoothing=0.0):
             logits = logits.float()
     labels = labels.contiguous().long()
     return _XentFn.apply(logits, labels, float(label_smoothing))
+
+
+# ------------------------------------------------------------------------------------------
+# Linear classifier + softmax cross-entropy in pieces of the vocabulary (csrc/linear_xent.hip): the
+# logits are never in memory as a whole, forward or backward.
+# ------------------------------------------------------------------------------------------
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def _counted(labels, V, ignore_index):
+    return (labels != ignore_index) & (labels >= 0) & (labels < V)
+
+
+def _linear_xent_plain(x, weight, labels, bias, smoothing, ignore_index, reduction):
+    """The same loss in torch operations: the rows that do not count are left out before the product."""
+    V = weight.shape[0]
+    keep = _counted(labels, V, ignore_index)
+    wide = torch.float64 if x.dtype == torch.float64 else F32
+    logits = TF.linear(x[keep].to(wide), weight.to(wide), bias.to(wide) if bias is not None else None)
+    rows = TF.cross_entropy(logits, labels[keep], reduction="none", label_smoothing=smoothing)
+    if reduction == "none":
+        return torch.zeros(labels.shape, dtype=wide, device=x.device).masked_scatter(keep, rows)
+    return rows.sum() / max(rows.numel(), 1) if reduction == "mean" else rows.sum()
+
+
+def _bf16_rows(t, D, Dp):
+    """``t`` [rows][D] as a bf16 operand of the products: rows of Dp columns (zeros behind D) on 16 bytes.
+    The tensor itself where it is one already."""
+    if t.dtype == BF16 and D == Dp and t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0 and \
+            D <= t.stride(0) <= 1 << 22:
+        return t
+    if t.stride(1) != 1 or t.stride(0) < D:
+        t = t.contiguous()
+    out = torch.empty((t.shape[0], Dp), dtype=BF16, device=t.device)
+    lib().pack_rows(ptr(t), int(t.dtype == BF16), t.stride(0), t.shape[0], D, ptr(out), Dp, stream_handle())
+    return out
+
+
+def _cached_weight(weight):
+    """fp32 parameters keep their bf16 operands from step to step (ops/wcache.py)."""
+    return weight.dtype == F32 and isinstance(weight, torch.nn.Parameter) and weight.is_contiguous()
+
+
+class _LinearXentFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, labels, smoothing, ignore_index, reduction):
+        with on_device(x):
+            track_leaves(ctx, x, weight, bias)
+            loss, ctx.cfg, saved = _linear_xent_forward(x, weight, bias, labels, smoothing, ignore_index, reduction, True)
+        ctx.save_for_backward(x, weight, bias, *saved)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, go):
+        x, weight, bias, labels, xk, wk, b, lse, total = ctx.saved_tensors
+        N, V, D, tail = ctx.cfg  # D: padded to whole K-tiles
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dev = x.device
+        sw = accumulation_sink(ctx, 1, weight) if need_w else None
+        sb = accumulation_sink(ctx, 2, bias) if need_b else None
+        dx = torch.empty((N, x.shape[1]), dtype=BF16, device=dev) if need_x else None
+        dw = sw if sw is not None else torch.empty(weight.shape, dtype=weight.dtype, device=dev) if need_w else None
+        db = sb if sb is not None else torch.empty(V, dtype=F32, device=dev) if need_b else None
+        go = go.detach().to(F32).reshape(-1).contiguous()
+        with on_device(x):
+            wt, Vp = None, (V + 63) // 64 * 64
+            if wk is None:
+                wk = _operand(weight, D)
+                if need_x and Vp <= 1 << 22:
+                    wt = _transposed_operand(weight, Vp)
+            args = (ptr(xk), xk.stride(0) if N > 1 else D, ptr(wk), wk.stride(0) if V > 1 else D, ptr(b), ptr(labels), N, V,
+                    D, x.shape[1], *tail)
+            nbytes = lib().linear_xent_bwd_bytes(*args, int(need_x), int(need_w), int(need_b), int(wt is not None))
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            lib().linear_xent_bwd(*args, ptr(go), ptr(total), ptr(ws), ptr(lse), ptr(wt), Vp, ptr(dx),
+                                  ptr(dw), int(weight.dtype == F32), int(sw is not None), ptr(db), int(sb is not None),
+                                  stream_handle())
+        return dx, None if sw is not None else dw, None if sb is not None else db, None, None, None, None
+
+
+def _operand(weight, Dp):
+    from .conv import _prep_weight
+
+    V, D = weight.shape
+    return _prep_weight(weight.view(V, D, 1, 1), 1, Dp, mode=0, param=weight).view(V, Dp)
+
+
+def _transposed_operand(weight, Vp):
+    from .conv import _prep_weight
+
+    V, D = weight.shape
+    return _prep_weight(weight.view(V, D, 1, 1), 1, Vp, mode=1, param=weight)
+
+
+def _linear_xent_forward(x, weight, bias, labels, smoothing, ignore_index, reduction, train):
+    N, D = x.shape
+    V, dev = weight.shape[0], x.device
+    Dp = (D + 63) // 64 * 64
+    xk = _bf16_rows(x.detach(), D, Dp)
+    cached = _cached_weight(weight)
+    wk = _operand(weight, Dp) if cached else _bf16_rows(weight.detach(), D, Dp)
+    b = bias.detach().contiguous() if bias is not None else None
+    tail = (ignore_index, smoothing, reduction)
+    args = (ptr(xk), xk.stride(0) if N > 1 else Dp, ptr(wk), wk.stride(0) if V > 1 else Dp, ptr(b), ptr(labels), N, V, Dp, D,
+            *tail)
+    ws = torch.empty(lib().linear_xent_fwd_bytes(*args), dtype=torch.uint8, device=dev)
+    lse = torch.empty(N, dtype=F32, device=dev) if train else None
+    rows = torch.empty(N, dtype=F32, device=dev) if reduction == 0 else None
+    total = torch.empty(2, dtype=F32, device=dev) if reduction else None
+    out = torch.empty((), dtype=F32, device=dev) if reduction else None
+    lib().linear_xent_fwd(*args, ptr(ws), ptr(lse), ptr(rows), ptr(total), ptr(out), stream_handle())
+    saved = (labels, xk, None if cached else wk, b, lse, total)
+    return (out if reduction else rows), (N, V, Dp, tail), saved
+
+
+def linear_cross_entropy(x, weight, labels, bias=None, label_smoothing=0.0, ignore_index=-100, reduction="mean"):
+    """Cross-entropy of ``softmax(x @ weight.T + bias)`` against ``labels``, with its gradients for x,
+    weight and bias, in pieces of the vocabulary: the logits are never kept (csrc/linear_xent.hip).
+
+    x (..., D) bf16 (fp32 is rounded to it, as ``linear`` does); weight (V, D) bf16, or the fp32
+    parameter, used through its bf16 operand; bias (V,) fp32 or None; labels (...) integers. Rows whose
+    label is ``ignore_index`` or lies outside [0, V) take no part: their loss and gradient are zero
+    whatever x holds there. ``reduction`` is "mean" over the rows that count (0 if none does), "sum",
+    or "none" (labels' shape). Products are summed in fp32, the loss and bias gradient are fp32, the
+    gradient of the logits is rounded to bf16 for the two products behind it; the weight's gradient
+    has the weight's type and goes straight into a live ``.grad`` buffer. At most 2^22 rows."""
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"linear_cross_entropy: reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError(f"linear_cross_entropy: x {tuple(x.shape)} does not match weight {tuple(weight.shape)} (V, D)")
+    if labels.shape != x.shape[:-1]:
+        raise ValueError(f"linear_cross_entropy: labels {tuple(labels.shape)} do not match x {tuple(x.shape)}")
+    if labels.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8):
+        raise TypeError(f"linear_cross_entropy: labels must be integers, got {labels.dtype}")
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise ValueError(f"linear_cross_entropy: bias has shape {tuple(bias.shape)}, expected ({weight.shape[0]},)")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"linear_cross_entropy: label_smoothing must lie in [0, 1], got {label_smoothing}")
+    same_device("linear_cross_entropy", x, weight, labels, bias)
+    D = x.shape[-1]
+    x2, flat = x.reshape(-1, D), labels.reshape(-1).long()
+    for name, t, kinds in (("x", x, (BF16, F32)), ("weight", weight, (BF16, F32)), ("bias", bias, (F32,))):
+        if t is not None and t.dtype not in kinds and native(x):
+            raise TypeError(f"linear_cross_entropy: {name} must be {' or '.join(str(k)[6:] for k in kinds)}, got {t.dtype}")
+    if not native(x) or not x2.shape[0]:
+        loss = _linear_xent_plain(x2, weight, flat, bias, float(label_smoothing), int(ignore_index), reduction)
+        return loss.reshape(labels.shape) if reduction == "none" else loss
+    if x2.shape[0] > int(lib().XENT_MAX_ROWS):
+        raise ValueError(f"linear_cross_entropy: {x2.shape[0]} rows, at most {int(lib().XENT_MAX_ROWS)} in a call")
+    if D > 1 << 22:
+        raise ValueError(f"linear_cross_entropy: rows of {D} values, at most {1 << 22}")
+    code = _REDUCTIONS[reduction]
+    if x2.dtype != BF16:
+        x2 = x2.to(BF16)
+    args = (x2, weight, bias, flat.contiguous(), float(label_smoothing), int(ignore_index), code)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, weight, bias)):
+        loss = _LinearXentFn.apply(*args)
+    else:
+        with on_device(x):
+            loss = _linear_xent_forward(x2, weight, bias, *args[3:], False)[0]
+    return loss if code else loss.reshape(labels.shape)
 
 
 # ------------------------------------------------------------------------------------------
