@@ -62,21 +62,30 @@ struct Vec<float> {
   }
 };
 
-// elements [c, c + E) of a row of D, zeros behind its end
-template <class T, int E = Vec<T>::E>
-DV_DEVICE void load_cols(const T* row, int c, int D, float (&v)[E]) {
-  if (c + E <= D) {
-    Vec<T>::unpack(Vec<T>::load(row + c), v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = c + e < D ? Vec<T>::get(row[c + e]) : 0.f;
+// the 16 bytes at element c of a row of D, zeros behind its end. Whole vectors only (TAIL false): no
+// branch, a lane behind the end reads the last one and drops it.
+template <class T, bool TAIL>
+DV_DEVICE u32x4 load_cols(const T* row, int c, int D) {
+  constexpr int E = Vec<T>::E;
+  if constexpr (!TAIL) {
+    const u32x4 r = Vec<T>::load(row + min(c, D - E));
+    return c < D ? r : u32x4{0, 0, 0, 0};
   }
+  if (c + E <= D) return Vec<T>::load(row + c);
+  u32x4 r{0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (c + e < D) {
+      if constexpr (sizeof(T) == 2) r[e >> 1] |= (uint32_t)row[c + e] << (16 * (e & 1));
+      else r[e] = __float_as_uint(row[c + e]);
+    }
+  return r;
 }
-template <class T, int E = Vec<T>::E>
+template <class T, bool TAIL, int E = Vec<T>::E>
 DV_DEVICE void store_cols(T* row, int c, int D, const float (&v)[E]) {
-  if (c + E <= D) {
+  if (TAIL ? c + E <= D : c < D) {
     Vec<T>::store(row + c, v);
-  } else {
+  } else if constexpr (TAIL) {
 #pragma unroll
     for (int e = 0; e < E; ++e)
       if (c + e < D) row[c + e] = Vec<T>::put(v[e]);
@@ -84,8 +93,17 @@ DV_DEVICE void store_cols(T* row, int c, int D, const float (&v)[E]) {
 }
 template <int E>
 DV_DEVICE void load_param(const float* w, int c, int D, float fill, float (&v)[E]) {
+  if (w && c + E <= D) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) v[e] = w && c + e < D ? w[c + e] : fill;
+    for (int q = 0; q < E / 4; ++q) {
+      const u32x4 r = *reinterpret_cast<const u32x4_a4*>(w + c + 4 * q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * q + e] = __uint_as_float(r[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = w && c + e < D ? w[c + e] : fill;
+  }
 }
 
 // sums of a and b over the LANES lanes of a row; LANES > 64 means the whole block
@@ -107,8 +125,9 @@ DV_DEVICE void row_sum2(float& a, float& b, float (*sh)[2]) {
 }
 
 constexpr int block_of(int lanes) { return lanes > 256 ? lanes : 256; }
+constexpr int bwd_block_of(int lanes) { return lanes == 64 ? 512 : block_of(lanes); }
 
-template <class T, int LANES, int VECS>
+template <class T, int LANES, int VECS, bool TAIL>
 __global__ __launch_bounds__(block_of(LANES)) void ln_fwd_kernel(const T* __restrict__ x, int64_t ldx,
                                                                  const float* __restrict__ w, const float* __restrict__ b,
                                                                  T* __restrict__ y, float* __restrict__ stats, int64_t rows,
@@ -123,11 +142,20 @@ __global__ __launch_bounds__(block_of(LANES)) void ln_fwd_kernel(const T* __rest
     load_param<E>(b, (lane + k * LANES) * E, D, 0.f, bv[k]);
   }
   const float inv = 1.f / D;
-  for (int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / LANES; r < rows; r += (int64_t)gridDim.x * RPB) {
+  u32x4 next[VECS];
+  int64_t r = (int64_t)blockIdx.x * RPB + threadIdx.x / LANES;
+  if (r < rows) {
+#pragma unroll
+    for (int k = 0; k < VECS; ++k) next[k] = load_cols<T, TAIL>(x + r * ldx, (lane + k * LANES) * E, D);
+  }
+  for (; r < rows; r += (int64_t)gridDim.x * RPB) {
     float v[VECS][E], s = 0.f, q = 0.f, none = 0.f;
 #pragma unroll
-    for (int k = 0; k < VECS; ++k) {
-      load_cols<T>(x + r * ldx, (lane + k * LANES) * E, D, v[k]);
+    for (int k = 0; k < VECS; ++k) Vec<T>::unpack(next[k], v[k]);
+    const int64_t r2 = r + (int64_t)gridDim.x * RPB;  // its loads run under this row's sums
+    if (r2 < rows) {
+#pragma unroll
+      for (int k = 0; k < VECS; ++k) next[k] = load_cols<T, TAIL>(x + r2 * ldx, (lane + k * LANES) * E, D);
     }
 #pragma unroll
     for (int k = 0; k < VECS; ++k)
@@ -149,52 +177,92 @@ __global__ __launch_bounds__(block_of(LANES)) void ln_fwd_kernel(const T* __rest
     for (int k = 0; k < VECS; ++k) {
 #pragma unroll
       for (int e = 0; e < E; ++e) v[k][e] = v[k][e] * rstd * wv[k][e] + bv[k][e];
-      store_cols<T>(y + r * D, (lane + k * LANES) * E, D, v[k]);
+      store_cols<T, TAIL>(y + r * D, (lane + k * LANES) * E, D, v[k]);
     }
   }
 }
 
-template <class T, int LANES, int VECS>
-__global__ __launch_bounds__(block_of(LANES)) void ln_bwd_kernel(const T* __restrict__ x, int64_t ldx,
-                                                                 const T* __restrict__ dy, int64_t ldg,
-                                                                 const float* __restrict__ w,
-                                                                 const float* __restrict__ stats, T* __restrict__ dx,
-                                                                 float* __restrict__ part, int64_t rows, int D) {
-  constexpr int E = Vec<T>::E, RPB = block_of(LANES) / LANES, COLS = LANES * VECS * E;
+template <class T, int LANES, int VECS, bool TAIL>
+__global__ __launch_bounds__(bwd_block_of(LANES)) void ln_bwd_kernel(const T* __restrict__ x, int64_t ldx,
+                                                                     const T* __restrict__ dy, int64_t ldg,
+                                                                     const float* __restrict__ w,
+                                                                     const float* __restrict__ stats, T* __restrict__ dx,
+                                                                     float* __restrict__ part, int64_t rows, int D) {
+  constexpr int E = Vec<T>::E, RPB = bwd_block_of(LANES) / LANES, COLS = LANES * VECS * E;
   __shared__ float sh[LANES > 64 ? LANES / 64 : 1][2];
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
-  float wv[VECS][E], aw[VECS][E] = {}, ab[VECS][E] = {};
+  float aw[VECS][E] = {}, ab[VECS][E] = {};
+  // w from LDS (the widest form: from cache) for every row: in registers it would spill the sums
+  constexpr bool W_LDS = COLS * 4 <= 32768;
+  __shared__ __attribute__((aligned(16))) float ws[W_LDS ? COLS : 4];
+  if constexpr (W_LDS) {
+    for (int c = threadIdx.x; c < COLS; c += bwd_block_of(LANES)) ws[c] = w && c < D ? w[c] : 1.f;
+    __syncthreads();
+  }
+  auto weight = [&](int k, float (&v)[E]) {
+    const int c = (lane + k * LANES) * E;
+    if constexpr (W_LDS) {
 #pragma unroll
-  for (int k = 0; k < VECS; ++k) load_param<E>(w, (lane + k * LANES) * E, D, 1.f, wv[k]);
+      for (int q = 0; q < E; q += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(ws + c + q);
+        v[q] = f.x; v[q + 1] = f.y; v[q + 2] = f.z; v[q + 3] = f.w;
+      }
+    } else {
+      load_param<E>(w, c, D, 1.f, v);
+    }
+  };
   const float inv = 1.f / D;
-  for (int64_t r = (int64_t)blockIdx.x * RPB + group; r < rows; r += (int64_t)gridDim.x * RPB) {
-    float v[VECS][E], g[VECS][E], s = 0.f, q = 0.f;
+  u32x4 nx[VECS], ng[VECS];
+  float2 nst{0.f, 0.f};
+  auto fetch = [&](int64_t r) {
 #pragma unroll
     for (int k = 0; k < VECS; ++k) {
-      load_cols<T>(x + r * ldx, (lane + k * LANES) * E, D, v[k]);
-      load_cols<T>(dy + r * ldg, (lane + k * LANES) * E, D, g[k]);
+      nx[k] = load_cols<T, TAIL>(x + r * ldx, (lane + k * LANES) * E, D);
+      ng[k] = load_cols<T, TAIL>(dy + r * ldg, (lane + k * LANES) * E, D);
     }
-    const float mu = stats[2 * r], rstd = stats[2 * r + 1];
+    nst = *reinterpret_cast<const float2*>(stats + 2 * r);
+  };
+  int64_t r = (int64_t)blockIdx.x * RPB + group;
+  if (r < rows) fetch(r);
+  for (; r < rows; r += (int64_t)gridDim.x * RPB) {
+    u32x4 cx[VECS], cg[VECS];
+    float s = 0.f, q = 0.f;
 #pragma unroll
-    for (int k = 0; k < VECS; ++k)
+    for (int k = 0; k < VECS; ++k) { cx[k] = nx[k]; cg[k] = ng[k]; }
+    const float mu = nst.x, rstd = nst.y;
+    const int64_t r2 = r + (int64_t)gridDim.x * RPB;  // its loads run under this row's sums
+    if (r2 < rows) fetch(r2);
+#pragma unroll
+    for (int k = 0; k < VECS; ++k) {
+      float v[E], g[E], wv[E];
+      Vec<T>::unpack(cx[k], v);
+      Vec<T>::unpack(cg[k], g);
+      weight(k, wv);
 #pragma unroll
       for (int e = 0; e < E; ++e) {  // behind the row's end g is 0, so every sum there adds nothing
-        v[k][e] = (v[k][e] - mu) * rstd;
-        aw[k][e] += g[k][e] * v[k][e];
-        ab[k][e] += g[k][e];
-        g[k][e] *= wv[k][e];
-        s += g[k][e];
-        q += g[k][e] * v[k][e];
+        v[e] = (v[e] - mu) * rstd;
+        aw[k][e] += g[e] * v[e];
+        ab[k][e] += g[e];
+        g[e] *= wv[e];
+        s += g[e];
+        q += g[e] * v[e];
       }
+    }
     row_sum2<LANES>(s, q, sh);
     s *= inv;
     q *= inv;
     if (dx) {
 #pragma unroll
       for (int k = 0; k < VECS; ++k) {
+        // from the packed words again: kept unpacked since the sums they would take twice the registers
+        asm volatile("" : "+v"(cx[k]), "+v"(cg[k]));
+        float v[E], g[E], wv[E];
+        Vec<T>::unpack(cx[k], v);
+        Vec<T>::unpack(cg[k], g);
+        weight(k, wv);
 #pragma unroll
-        for (int e = 0; e < E; ++e) g[k][e] = (g[k][e] - s - v[k][e] * q) * rstd;
-        store_cols<T>(dx + r * D, (lane + k * LANES) * E, D, g[k]);
+        for (int e = 0; e < E; ++e) g[e] = (g[e] * wv[e] - s - (v[e] - mu) * rstd * q) * rstd;
+        store_cols<T, TAIL>(dx + r * D, (lane + k * LANES) * E, D, g);
       }
     }
   }
@@ -223,7 +291,7 @@ __global__ __launch_bounds__(block_of(LANES)) void ln_bwd_kernel(const T* __rest
       }
       __syncthreads();
     }
-    for (int c = threadIdx.x; c < D; c += block_of(LANES)) {
+    for (int c = threadIdx.x; c < D; c += bwd_block_of(LANES)) {
       part[c] = fold[0][c];
       part[D + c] = fold[1][c];
     }
@@ -292,21 +360,41 @@ __global__ __launch_bounds__(256) void ln_param_wide_kernel(const T* __restrict_
   part[(int64_t)blockIdx.y * 2 * D + D + c] = ab;
 }
 
-// dw / db [D] (+)= sum over the slab's rows: 16 columns a block, 16 row lanes a column
+// dw / db [D] (+)= sum over the slab's rows: 16 columns a block (4 lanes of 16 bytes), 64 row lanes
 __global__ __launch_bounds__(256) void ln_fold_kernel(const float* __restrict__ part, int parts, int D,
                                                       float* __restrict__ dw, float* __restrict__ db, int acc_w, int acc_b) {
-  __shared__ float sh[16][17];
-  const int j = threadIdx.x & 15, i = threadIdx.x >> 4;
-  const int64_t c = (int64_t)blockIdx.x * 16 + j;
-  float s = 0.f;
-  if (c < 2 * (int64_t)D)
-    for (int p = i; p < parts; p += 16) s += part[(int64_t)p * 2 * D + c];
-  sh[i][j] = s;
+  __shared__ float sh[64][17];
+  __shared__ float half[16][17];
+  const int64_t width = 2 * (int64_t)D;
+  {
+    const int j = (threadIdx.x & 3) * 4, i = threadIdx.x >> 2;
+    const int64_t c = (int64_t)blockIdx.x * 16 + j;
+    float s[4] = {};
+    if (c + 4 <= width) {
+#pragma unroll 4
+      for (int p = i; p < parts; p += 64) {
+        const u32x4 r = *reinterpret_cast<const u32x4_a4*>(part + p * width + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[e] += __uint_as_float(r[e]);
+      }
+    } else {
+      for (int p = i; p < parts; p += 64)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e < width) s[e] += part[p * width + c + e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sh[i][j + e] = s[e];
+  }
   __syncthreads();
-  if (i == 0 && c < 2 * (int64_t)D) {
+  const int j = threadIdx.x & 15, i = threadIdx.x >> 4;
+  half[i][j] = (sh[4 * i][j] + sh[4 * i + 1][j]) + (sh[4 * i + 2][j] + sh[4 * i + 3][j]);
+  __syncthreads();
+  const int64_t c = (int64_t)blockIdx.x * 16 + j;
+  if (i == 0 && c < width) {
     float t = 0.f;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) t += sh[k][j];
+    for (int k = 0; k < 16; ++k) t += half[k][j];
     float* out = c < D ? dw : db;
     const int64_t o = c < D ? c : c - D;
     if (out) out[o] = (c < D ? acc_w : acc_b) ? out[o] + t : t;
@@ -315,14 +403,18 @@ __global__ __launch_bounds__(256) void ln_fold_kernel(const float* __restrict__ 
 
 constexpr int MAX_ELEMS = 32;  // fp32 values of a row a lane holds
 
-// f(LANES, VECS) of the narrowest form that holds D columns: the fewest lanes with at most
+// f(LANES, VECS, TAIL) of the narrowest form that holds D columns: the fewest lanes with at most
 // MAX_ELEMS values each, so that narrow rows share a wave
 template <class T, class F>
 bool with_form(int D, F&& f) {
   constexpr int E = Vec<T>::E, V = MAX_ELEMS / E;
   const int vecs = (D + E - 1) / E;
 #define LN_FORM(L, K) \
-  if (vecs <= (L) * (K)) { f(std::integral_constant<int, L>{}, std::integral_constant<int, K>{}); return true; }
+  if (vecs <= (L) * (K)) { \
+    if (D % E) f(std::integral_constant<int, L>{}, std::integral_constant<int, K>{}, std::true_type{}); \
+    else f(std::integral_constant<int, L>{}, std::integral_constant<int, K>{}, std::false_type{}); \
+    return true; \
+  }
   LN_FORM(16, 1)
   LN_FORM(32, 1)
   LN_FORM(64, 1)
@@ -340,10 +432,11 @@ bool with_form(int D, F&& f) {
 template <class T>
 void ln_fwd(const T* x, int64_t ldx, const float* w, const float* b, T* y, float* stats, int64_t rows, int D, float eps,
             hipStream_t st) {
-  const bool held = with_form<T>(D, [&](auto l, auto k) {
+  const bool held = with_form<T>(D, [&](auto l, auto k, auto t) {
     constexpr int L = decltype(l)::value, K = decltype(k)::value, RPB = block_of(L) / L;
-    const int64_t grid = std::min<int64_t>((rows + RPB - 1) / RPB, 256 * 8);
-    ln_fwd_kernel<T, L, K><<<(unsigned)grid, block_of(L), 0, st>>>(x, ldx, w, b, y, stats, rows, D, eps);
+    // as many blocks as run at once: each loads w and b once for all its rows
+    const int64_t grid = std::min<int64_t>((rows + RPB - 1) / RPB, 256 * (K * Vec<T>::E > 16 ? 3 : K * Vec<T>::E > 8 ? 5 : 8));
+    ln_fwd_kernel<T, L, K, decltype(t)::value><<<(unsigned)grid, block_of(L), 0, st>>>(x, ldx, w, b, y, stats, rows, D, eps);
   });
   if (!held) ln_fwd_wide_kernel<T><<<(unsigned)rows, 1024, 0, st>>>(x, ldx, w, b, y, stats, D, eps);
 }
@@ -351,9 +444,9 @@ void ln_fwd(const T* x, int64_t ldx, const float* w, const float* b, T* y, float
 template <class T>
 int ln_bwd(const T* x, int64_t ldx, const T* dy, int64_t ldg, const float* w, const float* stats, T* dx, float* part,
            int parts, int64_t rows, int D, hipStream_t st) {
-  const bool held = with_form<T>(D, [&](auto l, auto k) {
+  const bool held = with_form<T>(D, [&](auto l, auto k, auto t) {
     constexpr int L = decltype(l)::value, K = decltype(k)::value;
-    ln_bwd_kernel<T, L, K><<<(unsigned)parts, block_of(L), 0, st>>>(x, ldx, dy, ldg, w, stats, dx, part, rows, D);
+    ln_bwd_kernel<T, L, K, decltype(t)::value><<<(unsigned)parts, bwd_block_of(L), 0, st>>>(x, ldx, dy, ldg, w, stats, dx, part, rows, D);
   });
   if (!held) {
     if (dx) ln_bwd_wide_kernel<T><<<(unsigned)rows, 1024, 0, st>>>(x, ldx, dy, ldg, w, stats, dx, D);
@@ -366,12 +459,18 @@ int ln_bwd(const T* x, int64_t ldx, const T* dy, int64_t ldg, const float* w, co
 }
 }  // namespace
 
+// Blocks of the backward kernel = rows of its slab. Enough waves to cover the memory's latency (the
+// narrow forms hold less in flight a wave), few enough that the slab stays small beside the data.
 int dv_layer_norm_parts(int is_bf16, int64_t rows, int D) {
-  int per = 0;
-  auto rpb = [&](auto l, auto) { per = block_of(decltype(l)::value) / decltype(l)::value; };
-  const bool held = is_bf16 ? with_form<u16>(D, rpb) : with_form<float>(D, rpb);
+  int per = 0, most = 0;
+  auto form = [&](auto l, auto k, auto) {
+    constexpr int L = decltype(l)::value;
+    per = bwd_block_of(L) / L;
+    most = L < 64 ? 1536 : L == 64 ? (decltype(k)::value == 1 ? 512 : 256) : L == 256 ? 512 : 256;
+  };
+  const bool held = is_bf16 ? with_form<u16>(D, form) : with_form<float>(D, form);
   if (!held) return (int)std::min<int64_t>(rows, 64);
-  return (int)std::min<int64_t>((rows + per - 1) / per, 512);
+  return (int)std::min<int64_t>((rows + per - 1) / per, most);
 }
 
 int dv_layer_norm_fwd(const void* x, int is_bf16, int64_t ldx, const float* w, const float* b, void* y, float* stats,

@@ -16,25 +16,29 @@ from .common import BF16, F32, accumulation_sink, lib, native, on_device, ptr, s
 
 
 def _rows(t, D):
-    """``t`` as (rows, D) whose rows are dense and do not overlap; a view where the strides allow."""
-    t = t.reshape(-1, D)
-    if (D > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < D):
+    """(``t`` as (rows, D) whose rows are dense and do not overlap, row stride); a view where the strides allow."""
+    if t.dim() != 2:
+        t = t.reshape(-1, D)
+    s0, s1 = t.stride()
+    rows = t.shape[0]
+    if (s1 != 1 and D > 1) or (s0 < D and rows > 1):
         t = t.contiguous()
-    return t, (t.stride(0) if t.shape[0] > 1 else D)
+        s0 = D
+    return t, (s0 if rows > 1 else D)
 
 
-def _forward(x, weight, bias, eps, stats):
-    """(y, stats): per-row (mean, 1 / std) where a backward pass is going to need them."""
-    D = x.shape[-1]
-    x2, ld = _rows(x, D)
-    rows = x2.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((rows, 2), dtype=F32, device=x.device) if stats else None
-    w, b = (t.detach().contiguous() if t is not None else None for t in (weight, bias))
+def _dense(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _forward(x, ld, weight, bias, eps, train):
+    """(y, stats) of dense rows x: per-row (mean, 1 / std) where a backward pass is going to need them."""
+    rows, D = x.shape
+    y = torch.empty((rows, D), dtype=x.dtype, device=x.device)
+    stats = torch.empty((rows, 2), dtype=F32, device=x.device) if train else None
     if rows:
-        with on_device(x):
-            lib().layer_norm_fwd(ptr(x2), int(x.dtype == BF16), ld, ptr(w), ptr(b), ptr(y), ptr(stats), rows, D, eps,
-                                 stream_handle())
+        lib().layer_norm_fwd(ptr(x), int(x.dtype == BF16), ld, ptr(weight), ptr(bias), ptr(y), ptr(stats), rows, D, eps,
+                             stream_handle())
     return y, stats
 
 
@@ -43,34 +47,44 @@ class _LayerNormFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps):
         with on_device(x):
             track_leaves(ctx, x, weight, bias)
-        y, stats = _forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, bias, stats)
-        return y
+            x2, ctx.ld = _rows(x, x.shape[-1])
+            w = _dense(weight)
+            y, stats = _forward(x2, ctx.ld, w, _dense(bias), eps, True)
+        ctx.save_for_backward(x2, w, stats)
+        ctx.params = (weight, bias)  # leaves whose gradient may go straight into a live .grad
+        return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, stats = ctx.saved_tensors
-        D = x.shape[-1]
-        x2, ld = _rows(x, D)
-        g, ldg = _rows(dy if dy.dtype == x.dtype else dy.to(x.dtype), D)
-        rows, bf16 = x2.shape[0], int(x.dtype == BF16)
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        if not rows:
-            return (dx, torch.zeros_like(weight) if need_w else None, torch.zeros_like(bias) if need_b else None, None)
-        sinks = [accumulation_sink(ctx, i, t) if need else None
-                 for i, t, need in ((1, weight, need_w), (2, bias, need_b))]
-        dw, db = (s if s is not None else torch.empty(D, dtype=F32, device=x.device) if need else None
-                  for s, need in zip(sinks, (need_w, need_b)))
-        w = weight.detach().contiguous() if weight is not None else None
-        parts = lib().layer_norm_parts(bf16, rows, D)
-        part = torch.empty((parts, 2, D), dtype=F32, device=x.device) if need_w or need_b else None
-        with on_device(x):
-            lib().layer_norm_bwd(ptr(x2), bf16, ld, ptr(g), ldg, ptr(w), ptr(stats), ptr(dx), ptr(part), parts, ptr(dw),
-                                 ptr(db), int(sinks[0] is not None), int(sinks[1] is not None), rows, D, stream_handle())
-        dw, db = (None if s is not None or t is None else t for s, t in zip(sinks, (dw, db)))
-        return dx, dw, db, None
+        if torch.is_grad_enabled():
+            return _once(ctx, dy)
+        return _backward(ctx, dy)
+
+
+def _backward(ctx, dy):
+    x, w, stats = ctx.saved_tensors
+    weight, bias = ctx.params
+    rows, D = x.shape
+    dev, dtype = x.device, x.dtype
+    need_x, need_w, need_b, _ = ctx.needs_input_grad
+    dx = torch.empty(dy.shape, dtype=dtype, device=dev) if need_x else None
+    if not rows:
+        return dx, torch.zeros_like(weight) if need_w else None, torch.zeros_like(bias) if need_b else None, None
+    g, ldg = _rows(dy if dy.dtype == dtype else dy.to(dtype), D)
+    sw = accumulation_sink(ctx, 1, weight) if need_w else None
+    sb = accumulation_sink(ctx, 2, bias) if need_b else None
+    dw = sw if sw is not None else torch.empty(D, dtype=F32, device=dev) if need_w else None
+    db = sb if sb is not None else torch.empty(D, dtype=F32, device=dev) if need_b else None
+    bf16 = int(dtype == BF16)
+    parts = lib().layer_norm_parts(bf16, rows, D)
+    part = torch.empty(parts * 2 * D, dtype=F32, device=dev) if need_w or need_b else None
+    with on_device(x):
+        lib().layer_norm_bwd(ptr(x), bf16, ctx.ld, ptr(g), ldg, ptr(w), ptr(stats), ptr(dx), ptr(part), parts, ptr(dw), ptr(db),
+                             int(sw is not None), int(sb is not None), rows, D, stream_handle())
+    return dx, None if sw is not None else dw, None if sb is not None else db, None
+
+
+_once = torch.autograd.function.once_differentiable(_backward)  # create_graph=True: no second derivative
 
 
 def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
@@ -99,9 +113,9 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     if D == 0:
         raise ValueError("layer_norm: a normalized dimension is empty")
     if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias))):
-        if len(shape) > 1:
-            x = x.reshape(*x.shape[:-len(shape)], D)
-        return _forward(x, weight, bias, float(eps), False)[0].reshape(*x.shape[:-1], *shape)
+        with on_device(x):
+            x2, ld = _rows(x.detach(), D)
+            return _forward(x2, ld, _dense(weight), _dense(bias), float(eps), False)[0].view(x.shape)
     if len(shape) > 1:
         x2 = x.reshape(*x.shape[:-len(shape)], D)
         weight, bias = (t.reshape(D) if t is not None else None for t in (weight, bias))
