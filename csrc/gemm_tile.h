@@ -2,8 +2,13 @@
 // (k a multiple of 64, rows 16-byte aligned), fp32 sums in registers.
 //
 // A workgroup of WM x WN waves computes BM x BN; a wave TM x TN blocks of 32 x 32 with
-// v_mfma_f32_32x32x16_bf16. K-tiles of 64 go from global memory to a double-buffered LDS image by
-// LDS-DMA: the loads of tile t + 1 run under the products of tile t, one barrier a tile. An LDS row
+// v_mfma_f32_32x32x16_bf16. K-tiles of 64 go from global memory to two LDS images by
+// LDS-DMA. Fragments are read from LDS one step of 16 ahead of their products, across tiles too: the
+// barrier of a tile stands before its last step, whose fragments are in registers by then, so
+// the matrix cores have work while the first fragments of the next tile come. Half of a tile's loads are
+// issued behind that barrier and half in the next tile's first step: issued together they held
+// the products behind them up. 8192^3 with 256 x 256 tiles: 1360 TFLOP/s (the first form, every load
+// at the tile's start and the barrier at its end, 1218; the library's product 1473). An LDS row
 // is 128 bytes; its 16-byte chunks are exclusive-or swizzled by (row >> 1) & 7, so that the 16 lanes of
 // a ds_read_b128 cycle, 16 different rows, touch all 64 banks once.
 //
@@ -41,8 +46,12 @@ struct GemmTile {
                  : "v"(off), "s"(base), "s"(dst)
                  : "memory");
   }
-  static DV_DEVICE bf16x8 frag(const char* img, int r, int chunk) {
-    return *reinterpret_cast<const bf16x8*>(img + r * 128 + ((chunk ^ ((r >> 1) & 7)) << 4));
+  // this wave's LDS-DMA has landed and its LDS reads are done; then every wave's
+  static DV_DEVICE void landed() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x7 << 4);  // vmcnt(0) lgkmcnt(0); the builtin, which hipcc counts with
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
   }
 
   DV_DEVICE void run(const GemmOperand& a, const GemmOperand& b, int ktiles, char* smem) {
@@ -63,14 +72,33 @@ struct GemmTile {
       ob[i] = (uint32_t)(min(r, b.rows - 1) * b.ld * 2) + (((lane & 7) ^ ((r >> 1) & 7)) << 4);
     }
     const u16 *pa = a.p, *pb = b.p;
-    auto stage = [&](int buf) {
-      const uint32_t at = lds + buf * STAGE;
+    auto stage_a = [&](int slot) {
 #pragma unroll
-      for (int i = 0; i < IA; ++i) dma(pa, oa[i], at + (wave * IA + i) * 1024);
-#pragma unroll
-      for (int i = 0; i < IB; ++i) dma(pb, ob[i], at + BM * 128 + (wave * IB + i) * 1024);
+      for (int i = 0; i < IA; ++i) dma(pa, oa[i], lds + slot * STAGE + (wave * IA + i) * 1024);
       pa += BK;
+    };
+    auto stage_b = [&](int slot) {
+#pragma unroll
+      for (int i = 0; i < IB; ++i) dma(pb, ob[i], lds + slot * STAGE + BM * 128 + (wave * IB + i) * 1024);
       pb += BK;
+    };
+    // byte offset of this lane's fragment row, and its chunk swizzle (a row's 32 blocks share it)
+    const int ra = (wm * TM * 32 + (lane & 31)) * 128, rb = BM * 128 + (wn * TN * 32 + (lane & 31)) * 128;
+    const int swz = ((lane & 31) >> 1) & 7, half = lane >> 5;
+    bf16x8 fa[2][TM], fb[2][TN];
+    auto read = [&](int f, int slot, int k) {
+      const char* img = smem + slot * STAGE + (((k * 2 + half) ^ swz) << 4);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) fb[f][j] = *reinterpret_cast<const bf16x8*>(img + rb + j * 32 * 128);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) fa[f][i] = *reinterpret_cast<const bf16x8*>(img + ra + i * 32 * 128);
+    };
+    auto multiply = [&](int f) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[f][i], fb[f][j], acc[i][j], 0, 0, 0);
     };
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -78,28 +106,39 @@ struct GemmTile {
       for (int j = 0; j < TN; ++j)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    stage(0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    for (int t = 0; t < ktiles; ++t) {
-      const int cur = t & 1;
-      if (t + 1 < ktiles) stage(cur ^ 1);
-      const char* ia = smem + cur * STAGE;
-      const char* ib = ia + BM * 128;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        bf16x8 fa[TM], fb[TN];
-#pragma unroll
-        for (int i = 0; i < TM; ++i) fa[i] = frag(ia, (wm * TM + i) * 32 + (lane & 31), k * 2 + (lane >> 5));
-#pragma unroll
-        for (int j = 0; j < TN; ++j) fb[j] = frag(ib, (wn * TN + j) * 32 + (lane & 31), k * 2 + (lane >> 5));
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j], acc[i][j], 0, 0, 0);
-      }
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      __syncthreads();
+    stage_a(0);
+    stage_b(0);
+    if (ktiles > 1) stage_a(1);
+    landed();
+    read(0, 0, 0);
+    // the scheduling barriers keep a step's reads before its products: hipcc sinks them to save registers
+    auto tile = [&](int t, int cur, int nxt) {
+      read(1, cur, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      if (t + 1 < ktiles) stage_b(nxt);  // of tile t + 1
+      multiply(0);
+      __builtin_amdgcn_sched_barrier(0);
+      read(0, cur, 2);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(1);
+      __builtin_amdgcn_sched_barrier(0);
+      read(1, cur, 3);
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(0);
+      __builtin_amdgcn_sched_barrier(0);
+      landed();  // tile t's fragments are in registers, its slot is free; tile t + 1 is in LDS
+      if (t + 1 < ktiles) read(0, nxt, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (t + 2 < ktiles) stage_a(cur);
+      multiply(1);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    int t = 0;
+    for (; t + 1 < ktiles; t += 2) {
+      tile(t, 0, 1);
+      tile(t + 1, 1, 0);
     }
+    if (t < ktiles) tile(t, 0, 1);
+    landed();  // LDS is free for the caller
   }
 };

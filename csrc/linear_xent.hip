@@ -55,20 +55,34 @@ DV_DEVICE float common_scale(const DvXent& a) {
   return a.reduction == DV_XENT_NONE ? 1.f : a.reduction == DV_XENT_SUM ? a.go[0] : a.go[0] / fmaxf(a.total[1], 1.f);
 }
 
-// acc + bias, -inf behind the last class; `last`: the tile holds columns behind it
-template <class T>
+// exp(a - b) as exp2((a - b) * LOG2E): subtracted first, since a class ruled out by the type's lowest
+// value leaves the type's range where the product comes first
+constexpr float LOG2E = 1.44269504f;
+DV_DEVICE float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// acc + bias, -inf behind the last class
+template <class T, int BM>
 DV_DEVICE void add_bias(T& t, const DvXent& a, int v0) {
-  const bool last = v0 + T::TM * 32 * 8 > a.V;  // (conservative: any tile near the end)
-  if (!a.bias && !last) return;
+  if (a.bias) {
 #pragma unroll
-  for (int i = 0; i < T::TM; ++i)
+    for (int i = 0; i < T::TM; ++i) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int v = v0 + t.row(i, r);
-      const float b = a.bias && v < a.V ? a.bias[v] : 0.f;
+      for (int r = 0; r < 16; ++r) {
+        const float b = a.bias[min(v0 + t.row(i, r), a.V - 1)];
 #pragma unroll
-      for (int j = 0; j < T::TN; ++j) t.acc[i][j][r] = v < a.V ? t.acc[i][j][r] + b : -INFINITY;
+        for (int j = 0; j < T::TN; ++j) t.acc[i][j][r] += b;
+      }
+      __builtin_amdgcn_sched_barrier(0);  // 16 loads at a time: all of them at once spill
     }
+  }
+  if (v0 + BM > a.V) {
+#pragma unroll
+    for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int j = 0; j < T::TN; ++j) t.acc[i][j][r] = v0 + t.row(i, r) < a.V ? t.acc[i][j][r] : -INFINITY;
+  }
 }
 
 // ---------------------------------------------------------------------------------------- forward
@@ -82,33 +96,39 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void stats_kernel(D
   const int v0 = at.m * BM, n0 = at.n * BN;
   T t;
   t.run({a.w + (int64_t)v0 * a.ldw, a.ldw, a.V - v0}, {a.x + (int64_t)n0 * a.ldx, a.ldx, a.N - n0}, a.D / 64, smem);
-  add_bias(t, a, v0);
+  add_bias<T, BM>(t, a, v0);
+  const int vw = v0 + t.wm * T::TM * 32;  // the wave's columns: [vw, vw + 32 TM)
 #pragma unroll
   for (int j = 0; j < T::TN; ++j) {
     const int n = n0 + t.col(j);
     const int64_t label = n < a.N ? a.labels[n] : -1;
-    const bool use = counted(label, a);
-    float top = -INFINITY, s = 0.f, sum = 0.f;
+    const bool here = counted(label, a) && label >= vw && label < vw + T::TM * 32;
+    if (__any(here)) {  // few of many pieces of the vocabulary hold a label of the wave's rows
+      const int rel = here ? (int)label - vw - 4 * (t.lane >> 5) : -1;
+#pragma unroll
+      for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (rel == i * 32 + (r & 3) + 8 * (r >> 2)) at_label[n] = t.acc[i][j][r];
+    }
+    float top = -INFINITY, s = 0.f;
 #pragma unroll
     for (int i = 0; i < T::TM; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float l = t.acc[i][j][r];
-        top = fmaxf(top, l);
-        if (use && v0 + t.row(i, r) == (int)label) at_label[n] = l;
-      }
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, t.acc[i][j][r]);
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
     for (int i = 0; i < T::TM; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s += __expf(t.acc[i][j][r] - ref);
+      for (int r = 0; r < 16; ++r) s += exp2_fast((t.acc[i][j][r] - ref) * LOG2E);
     s += __shfl_xor(s, 32, 64);
+    float sum = 0.f;
     if (psum) {
 #pragma unroll
       for (int i = 0; i < T::TM; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sum += v0 + t.row(i, r) < a.V ? t.acc[i][j][r] : 0.f;
+        for (int r = 0; r < 16; ++r) sum += v0 + t.row(i, r) < a.V ? t.acc[i][j][r] - ref : 0.f;
       sum += __shfl_xor(sum, 32, 64);
     }
     if (t.lane < 32 && n < a.N) {
@@ -119,52 +139,71 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void stats_kernel(D
   }
 }
 
-// 64 rows a block, 16 strips of the parts: lse and the row's loss; the block's (sum, count)
+// ROWS rows a block, 1024 / ROWS strips of the parts: (largest logit, log2 of the sum of exponentials
+// above it) of each row, kept apart so that a large common offset costs no precision, and its loss; the block's (sum, count),
+// or where one block holds every row the result itself
+template <int ROWS>
 __global__ __launch_bounds__(1024) void join_kernel(DvXent a, const float2* __restrict__ part, const float* __restrict__ psum,
-                                                    const float* __restrict__ at_label, int parts,
-                                                    float* __restrict__ lse, float* __restrict__ loss,
-                                                    float2* __restrict__ blocks) {
-  __shared__ float sh[3][16][64];
-  const int j = threadIdx.x & 63, k = threadIdx.x >> 6;
-  const int64_t n = (int64_t)blockIdx.x * 64 + j;
-  float m = -INFINITY, s = 0.f, sum = 0.f;
+                                                    const float* __restrict__ at_label, int parts, int cols_a_part,
+                                                    float2* __restrict__ lse, float* __restrict__ loss,
+                                                    float2* __restrict__ blocks, float* __restrict__ out,
+                                                    float* __restrict__ total) {
+  constexpr int STRIPS = 1024 / ROWS;
+  __shared__ float sh[3][STRIPS][ROWS];
+  __shared__ float red[2][ROWS / 64];
+  const int j = threadIdx.x % ROWS, k = threadIdx.x / ROWS;
+  const int64_t n = (int64_t)blockIdx.x * ROWS + j;
+  float top = -INFINITY;
   if (n < a.N)
-    for (int p = k; p < parts; p += 16) {
+    for (int p = k; p < parts; p += STRIPS) top = fmaxf(top, part[(int64_t)p * a.N + n].x);
+  sh[0][k][j] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < STRIPS; ++i) top = fmaxf(top, sh[0][i][j]);
+  float s = 0.f, sum = 0.f;  // of exp(l - top), of l - top
+  if (n < a.N)
+    for (int p = k; p < parts; p += STRIPS) {
       const float2 q = part[(int64_t)p * a.N + n];
-      const float t = fmaxf(m, q.x);
-      if (t != -INFINITY) s = s * __expf(m - t) + q.y * __expf(q.x - t);
-      else s += q.y;  // nothing but -inf so far (q.y is 0), or NaN
-      m = t;
-      if (psum) sum += psum[(int64_t)p * a.N + n];
+      s += q.x == -INFINITY ? q.y : q.y * exp2_fast((q.x - top) * LOG2E);  // (-inf: 0, or NaN)
+      if (psum) {
+        const int cols = min(a.V - p * cols_a_part, cols_a_part);
+        if (cols > 0) sum += psum[(int64_t)p * a.N + n] + (q.x == -INFINITY ? 0.f : cols * (q.x - top));
+      }
     }
-  sh[0][k][j] = m;
   sh[1][k][j] = s;
   sh[2][k][j] = sum;
   __syncthreads();
-  if (k) return;
-  float top = -INFINITY, tot = 0.f, all = 0.f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) top = fmaxf(top, sh[0][i][j]);
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    tot += top == -INFINITY ? sh[1][i][j] : sh[1][i][j] * __expf(sh[0][i][j] - top);
-    all += sh[2][i][j];
-  }
   float l = 0.f, one = 0.f;
-  if (n < a.N) {
-    const float z = top + logf(tot);
-    if (counted(a.labels[n], a)) {
-      one = 1.f;
-      l = z - (1.f - a.smooth) * at_label[n];
-      if (psum) l -= a.smooth * (all / a.V);
+  if (k == 0) {
+    float tot = 0.f, all = 0.f;
+#pragma unroll
+    for (int i = 0; i < STRIPS; ++i) { tot += sh[1][i][j]; all += sh[2][i][j]; }
+    if (n < a.N) {
+      if (counted(a.labels[n], a)) {
+        one = 1.f;
+        l = logf(tot) + (1.f - a.smooth) * (top - at_label[n]);
+        if (psum) l -= a.smooth * (all / a.V);
+      }
+      if (lse) lse[n] = {top, log2f(tot)};
+      if (loss) loss[n] = l;
     }
-    if (lse) lse[n] = z;
-    if (loss) loss[n] = l;
   }
-  if (blocks) {
-    l = wave_sum(l);
-    one = wave_sum(one);
-    if (j == 0) blocks[blockIdx.x] = {l, one};
+  if (!out) return;
+  l = wave_sum(l);
+  one = wave_sum(one);
+  if (k == 0 && (j & 63) == 0) { red[0][j >> 6] = l; red[1][j >> 6] = one; }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    l = one = 0.f;
+#pragma unroll
+    for (int i = 0; i < ROWS / 64; ++i) { l += red[0][i]; one += red[1][i]; }
+    if (gridDim.x > 1) {
+      blocks[blockIdx.x] = {l, one};
+    } else {
+      total[0] = l;
+      total[1] = one;
+      *out = a.reduction == DV_XENT_MEAN ? l / fmaxf(one, 1.f) : l;
+    }
   }
 }
 
@@ -187,7 +226,7 @@ __global__ __launch_bounds__(256) void total_kernel(const float2* __restrict__ b
 // d of the piece [p0, p0 + pv) of the vocabulary: P [n][ldp], zero up to pvp columns, and
 // Q = t . d [v][ldq], zero up to ldq; db partial sums [n block and wave][pv]
 template <class T, int BM, int BN, int WN>
-__global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(DvXent a, const float* __restrict__ lse, int p0,
+__global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(DvXent a, const float2* __restrict__ lse, int p0,
                                                                               int pv, int pvp, u16* __restrict__ P,
                                                                               u16* __restrict__ Q, int64_t ldq,
                                                                               float* __restrict__ pbias) {
@@ -199,25 +238,41 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(Dv
   const int v0 = at.m * BM, n0 = at.n * BN;  // v: within the piece
   T t;
   t.run({a.w + (int64_t)(p0 + v0) * a.ldw, a.ldw, pv - v0}, {a.x + (int64_t)n0 * a.ldx, a.ldx, a.N - n0}, a.D / 64, smem);
-  add_bias(t, a, p0 + v0);
+  add_bias<T, BM>(t, a, p0 + v0);
   const float off = a.smooth / a.V, hot = 1.f - a.smooth;
+  const int vw0 = p0 + v0 + t.wm * T::TM * 32;
   float ts[T::TN];
 #pragma unroll
   for (int j = 0; j < T::TN; ++j) {
     const int n = n0 + t.col(j);
     const int64_t label = n < a.N ? a.labels[n] : -1;
     const bool use = n < a.N && counted(label, a);
-    const float z = use ? lse[n] : 0.f;
+    const float2 z = use ? lse[n] : float2{0.f, 0.f};
     ts[j] = use ? (a.reduction == DV_XENT_NONE ? a.go[n] : 1.f) : 0.f;
 #pragma unroll
     for (int i = 0; i < T::TM; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int v = p0 + v0 + t.row(i, r);
-        float d = __expf(t.acc[i][j][r] - z) - off;
-        if (v == (int)label) d -= hot;
-        t.acc[i][j][r] = use && v < p0 + pv ? d : 0.f;
-      }
+      for (int r = 0; r < 16; ++r) t.acc[i][j][r] = exp2_fast(fmaf(t.acc[i][j][r] - z.x, LOG2E, -z.y)) - off;
+    const bool here = use && label >= vw0 && label < vw0 + T::TM * 32;
+    if (__any(here)) {
+      const int rel = here ? (int)label - vw0 - 4 * (t.lane >> 5) : -1;
+#pragma unroll
+      for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t.acc[i][j][r] -= rel == i * 32 + (r & 3) + 8 * (r >> 2) ? hot : 0.f;
+    }
+    if (__any(!use)) {  // whatever x holds in rows that do not count
+#pragma unroll
+      for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t.acc[i][j][r] = use ? t.acc[i][j][r] : 0.f;
+    }
+    if (v0 + BM > pv) {  // behind the piece's end
+#pragma unroll
+      for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t.acc[i][j][r] = v0 + t.row(i, r) < pv ? t.acc[i][j][r] : 0.f;
+    }
   }
   if (pbias) {  // over the wave's rows n: in registers, then over the 32 lanes of a column of blocks
 #pragma unroll
@@ -235,9 +290,11 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(Dv
   }
   // both layouts through this wave's own part of LDS, MW columns of the vocabulary at a time
   char* mine = smem + t.wave * (NW > MW ? NW : MW) * PITCH;
+  const uint32_t swap = t.lane & 1 ? 0x07060302u : 0x01000504u;
 #pragma unroll
   for (int h = 0; h < T::TM / MG; ++h) {
     const int vw = v0 + (t.wm * T::TM + h * MG) * 32, nw = n0 + t.wn * T::TN * 32;
+    uint32_t u[MG][T::TN][8];  // pairs of columns v of this lane's row n
 #pragma unroll
     for (int j = 0; j < T::TN; ++j)
 #pragma unroll
@@ -245,13 +302,15 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(Dv
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const f32x16& c = t.acc[h * MG + i][j];
-          const uint2 d{pack2bf(c[4 * q], c[4 * q + 1]), pack2bf(c[4 * q + 2], c[4 * q + 3])};
-          *reinterpret_cast<uint2*>(mine + (j * 32 + (t.lane & 31)) * PITCH + (i * 32 + 8 * q + 4 * (t.lane >> 5)) * 2) = d;
+          u[i][j][2 * q] = pack2bf(c[4 * q], c[4 * q + 1]);
+          u[i][j][2 * q + 1] = pack2bf(c[4 * q + 2], c[4 * q + 3]);
+          *reinterpret_cast<uint2*>(mine + (j * 32 + (t.lane & 31)) * PITCH + (i * 32 + 8 * q + 4 * (t.lane >> 5)) * 2) =
+              uint2{u[i][j][2 * q], u[i][j][2 * q + 1]};
         }
     wave_sync();
 #pragma unroll
     for (int e = 0; e < NW * MW / 512; ++e) {
-      const int u = e * 64 + t.lane, n = u / (MW / 8), c = u % (MW / 8) * 8;
+      const int w = e * 64 + t.lane, n = w / (MW / 8), c = w % (MW / 8) * 8;
       const uint4 d = *reinterpret_cast<const uint4*>(mine + n * PITCH + c * 2);
       if (nw + n < a.N && vw + c < pvp) *reinterpret_cast<uint4*>(P + (int64_t)(nw + n) * pvp + vw + c) = d;
     }
@@ -262,14 +321,20 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(Dv
 #pragma unroll
         for (int i = 0; i < MG; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int v = i * 32 + (r & 3) + 8 * (r >> 2) + 4 * (t.lane >> 5);
-            *reinterpret_cast<u16*>(mine + v * PITCH + (j * 32 + (t.lane & 31)) * 2) = f2bf(t.acc[h * MG + i][j][r] * ts[j]);
+          for (int k = 0; k < 8; ++k) {  // columns v, v + 1 of two neighbouring rows n become rows of Q
+            uint32_t w = u[i][j][k];
+            if (a.reduction == DV_XENT_NONE) {
+              const f32x16& c = t.acc[h * MG + i][j];
+              w = pack2bf(c[2 * k] * ts[j], c[2 * k + 1] * ts[j]);
+            }
+            const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0xB1, 0xF, 0xF, false);  // lane ^ 1
+            const int v = i * 32 + (k & 1) * 2 + 8 * (k >> 1) + 4 * (t.lane >> 5) + (t.lane & 1);
+            *reinterpret_cast<uint32_t*>(mine + v * PITCH + (j * 32 + (t.lane & 30)) * 2) = __builtin_amdgcn_perm(w, o, swap);
           }
       wave_sync();
 #pragma unroll
       for (int e = 0; e < NW * MW / 512; ++e) {
-        const int u = e * 64 + t.lane, v = u / (NW / 8), c = u % (NW / 8) * 8;
+        const int w = e * 64 + t.lane, v = w / (NW / 8), c = w % (NW / 8) * 8;
         const uint4 d = *reinterpret_cast<const uint4*>(mine + v * PITCH + c * 2);
         if (vw + v < pv && nw + c < ldq) *reinterpret_cast<uint4*>(Q + (int64_t)(vw + v) * ldq + nw + c) = d;
       }
@@ -314,14 +379,41 @@ DV_DEVICE void put4(void* out, int f32, int add, int64_t o, int left, f32x4 v) {
   }
 }
 
+// db[v] (+)= scale * sum of the partial rows, 64 columns a block
+struct BiasArgs {
+  const float* part;
+  int parts, pv;
+  float* db;
+  int add;
+};
+DV_DEVICE void fold_bias(const DvXent& x, const BiasArgs& b, int block, float* sh) {
+  const int j = threadIdx.x & 63, k = threadIdx.x >> 6, v = block * 64 + j;
+  float s = 0.f;
+  if (v < b.pv && k < 4)
+    for (int p = k; p < b.parts; p += 4) s += b.part[(int64_t)p * b.pv + v];
+  if (k < 4) sh[k * 64 + j] = s;
+  __syncthreads();
+  if (k == 0 && v < b.pv) {
+    s = ((sh[j] + sh[64 + j]) + (sh[128 + j] + sh[192 + j])) * common_scale(x);
+    b.db[v] = b.add ? b.db[v] + s : s;
+  }
+}
+
+// The products behind a piece's d, and the fold of its bias gradient, in one launch: blocks
+// [0, b0) compute g0, [b0, b0 + b1) g1, the rest the bias.
 template <class T, int BM, int BN>
-__global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void out_kernel(DvXent x, OutArgs g) {
+__global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void out_kernel(DvXent x, OutArgs g0, OutArgs g1, BiasArgs bias,
+                                                                             int b0, int b1) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int PITCH = 144, NW = 32 * T::TN;
+  int id = blockIdx.x;
+  if (id >= b0 + b1) return fold_bias(x, bias, id - b0 - b1, reinterpret_cast<float*>(smem));
+  const bool second = id >= b0;
+  const OutArgs& g = second ? g1 : g0;
+  if (second) id -= b0;
   const int tm = (g.M + BM - 1) / BM, tn = (g.N + BN - 1) / BN;
-  // splits of one tile sit next to each other in the grid only where tiles are few; whole tiles first
-  const int tiles = tm * tn, split = blockIdx.x / tiles;
-  const TileAt at = tile_at(blockIdx.x - split * tiles, tiles, tm, tn);
+  const int tiles = tm * tn, split = id / tiles;
+  const TileAt at = tile_at(id - split * tiles, tiles, tm, tn);
   const int m0 = at.m * BM, n0 = at.n * BN;
   const int k0 = (int)((int64_t)g.ktiles * split / g.splits), k1 = (int)((int64_t)g.ktiles * (split + 1) / g.splits);
   T t;
@@ -378,36 +470,40 @@ __global__ __launch_bounds__(256) void reduce_kernel(DvXent x, OutArgs g) {
   }
 }
 
-// db[v] (+)= scale * sum of the partial rows
-__global__ __launch_bounds__(256) void bias_kernel(DvXent x, const float* __restrict__ part, int parts, int pv,
-                                                   float* __restrict__ db, int add) {
-  __shared__ float sh[4][64];
-  const int j = threadIdx.x & 63, k = threadIdx.x >> 6, v = blockIdx.x * 64 + j;
-  float s = 0.f;
-  if (v < pv)
-    for (int p = k; p < parts; p += 4) s += part[(int64_t)p * pv + v];
-  sh[k][j] = s;
-  __syncthreads();
-  if (k == 0 && v < pv) {
-    s = ((sh[0][j] + sh[1][j]) + (sh[2][j] + sh[3][j])) * common_scale(x);
-    db[v] = add ? db[v] + s : s;
+// dst[c][r] = src[r][c] for r < rows (by_label: only of counted rows), 0 up to ldd; 64 x 64 a block, one
+// or two matrices a launch. 16-byte loads and stores; a column of the LDS image is gathered by 2 bytes.
+struct Transpose {
+  const u16* src;
+  int64_t ld;
+  int rows, cols;
+  u16* dst;
+  int64_t ldd;
+  int by_label;
+  int blocks;  // (ldd / 64) x ceil(cols / 64)
+};
+__global__ __launch_bounds__(256) void transpose_kernel(DvXent x, Transpose m0, Transpose m1) {
+  __shared__ __attribute__((aligned(16))) u16 sh[64][74];  // 37 banks a row: gathers of 8 rows apart do not meet
+  int id = blockIdx.x;
+  const Transpose& t = id < m0.blocks ? m0 : m1;
+  if (id >= m0.blocks) id -= m0.blocks;
+  const int across = (int)(t.ldd / 64), r0 = id % across * 64, c0 = id / across * 64;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {  // rows of the operand hold whole 64-column blocks (zeros from `width` on)
+    const int r = e * 32 + (threadIdx.x >> 3), c = (threadIdx.x & 7) * 8;
+    uint4 d{0, 0, 0, 0};
+    if (r0 + r < t.rows && (!t.by_label || counted(x.labels[r0 + r], x)))
+      d = *reinterpret_cast<const uint4*>(t.src + (int64_t)(r0 + r) * t.ld + c0 + c);
+    uint32_t* to = reinterpret_cast<uint32_t*>(&sh[r][c]);
+    to[0] = d.x; to[1] = d.y; to[2] = d.z; to[3] = d.w;
   }
-}
-
-// dst[c][r] = src[r][c] for r < rows (labels given: only of counted rows), 0 up to ldd; 64 x 64 a block
-__global__ __launch_bounds__(256) void transpose_kernel(DvXent x, const u16* __restrict__ src, int64_t lds_, int rows, int cols,
-                                                        u16* __restrict__ dst, int64_t ldd, int by_label) {
-  __shared__ u16 sh[64][66];
-  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
-  for (int e = threadIdx.x; e < 4096; e += 256) {
-    const int r = e >> 6, c = e & 63;
-    const bool in = r0 + r < rows && c0 + c < cols && (!by_label || counted(x.labels[r0 + r], x));
-    sh[r][c] = in ? src[(int64_t)(r0 + r) * lds_ + c0 + c] : (u16)0;
-  }
   __syncthreads();
-  for (int e = threadIdx.x; e < 4096; e += 256) {
-    const int c = e >> 6, r = e & 63;
-    if (c0 + c < cols && r0 + r < ldd) dst[(int64_t)(c0 + c) * ldd + r0 + r] = sh[r][c];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int c = e * 32 + (threadIdx.x >> 3), r = (threadIdx.x & 7) * 8;
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = (uint32_t)sh[r + 2 * k][c] | (uint32_t)sh[r + 2 * k + 1][c] << 16;
+    if (c0 + c < t.cols) *reinterpret_cast<uint4*>(t.dst + (int64_t)(c0 + c) * t.ldd + r0 + r) = uint4{w[0], w[1], w[2], w[3]};
   }
 }
 
@@ -437,20 +533,25 @@ __global__ __launch_bounds__(256) void pack_kernel(const S* __restrict__ src, in
 // ------------------------------------------------------------------------------------------- host
 // Tile and split of an M x N x (64 ktiles) product: the least time by a model of one K-tile's time on
 // a full CU (throughput) and alone (latency), both measured.
-struct Plan { int form, splits; };
+struct Plan { int form, splits; double us; };
 constexpr int FORM_TILE[3] = {256, 128, 64};
-Plan plan(int64_t M, int64_t N, int ktiles, bool may_split) {
-  constexpr double FULL[3] = {1.7, 0.58, 0.25}, ALONE[3] = {1.7, 0.8, 0.5};  // us a K-tile
-  Plan best{0, 1};
-  double least = 1e30;
-  for (int f = 0; f < 3; ++f) {
-    const int64_t tiles = (int64_t)cdiv(M, FORM_TILE[f]) * cdiv(N, FORM_TILE[f]);
-    for (int s = 1; s <= (may_split ? std::min(ktiles, 32) : 1); ++s) {
-      const double k = cdiv(ktiles, s), blocks = (double)tiles * s;
-      const double per_cu = f == 0 ? std::ceil(blocks / 256) : std::max(1.0, blocks / 256);
-      const double us = std::max(per_cu * k * FULL[f], k * ALONE[f]) + (s > 1 ? 3.0 + s * (double)M * N * 8 / 4e6 : 0.0);
-      if (us < least) { least = us; best = {f, s}; }
-    }
+Plan plan_form(int f, int64_t M, int64_t N, int ktiles, bool may_split) {
+  constexpr double FULL[3] = {1.6, 0.58, 0.25}, ALONE[3] = {1.6, 0.65, 0.35};  // us a K-tile
+  Plan best{f, 1, 1e30};
+  const int64_t tiles = (int64_t)cdiv(M, FORM_TILE[f]) * cdiv(N, FORM_TILE[f]);
+  for (int s = 1; s <= (may_split ? std::min(ktiles, 32) : 1); ++s) {
+    const double k = cdiv(ktiles, s), blocks = (double)tiles * s;
+    const double per_cu = f == 0 ? std::ceil(blocks / 256) : std::max(1.0, blocks / 256);
+    const double us = std::max(per_cu * k * FULL[f], k * ALONE[f]) + (s > 1 ? 4.0 + s * (double)M * N * 8 / 4e6 : 0.0);
+    if (us < best.us) best = {f, s, us};
+  }
+  return best;
+}
+Plan plan(int64_t M, int64_t N, int ktiles) {
+  Plan best = plan_form(0, M, N, ktiles, false);
+  for (int f = 1; f < 3; ++f) {
+    const Plan p = plan_form(f, M, N, ktiles, false);
+    if (p.us < best.us) best = p;
   }
   return best;
 }
@@ -473,12 +574,13 @@ void allow_lds(K kernel, int bytes, bool (&done)[64]) {
   done[dev & 63] = true;
 }
 
-struct FwdLayout { Plan p; int parts, blocks; int64_t part, psum, label, block, bytes; };
+struct FwdLayout { Plan p; int parts, rows, blocks; int64_t part, psum, label, block, bytes; };
 FwdLayout fwd_layout(const DvXent& a) {
   FwdLayout l;
-  l.p = plan(a.V, a.N, a.D / 64, false);
+  l.p = plan(a.V, a.N, a.D / 64);
   l.parts = cdiv(a.V, FORM_TILE[l.p.form]) * FORM_WM[l.p.form];
-  l.blocks = cdiv(a.N, 64);
+  l.rows = a.N <= 256 && l.parts <= 128 ? 256 : 64;  // small: one block joins every row
+  l.blocks = cdiv(a.N, l.rows);
   int64_t at = 0;
   auto take = [&](int64_t b) { const int64_t o = at; at += up(b, 256); return o; };
   l.part = take((int64_t)l.parts * a.N * 8);
@@ -504,9 +606,14 @@ BwdLayout bwd_layout(const DvXent& a, bool need_x, bool need_w, bool need_b, boo
   const int64_t most = std::max<int64_t>(PIECE_BYTES / (4 * l.ldq) / 256 * 256, 256);
   const int pieces = cdiv(a.V, most);
   l.piece = (int)std::min<int64_t>(up(cdiv(a.V, pieces), 256), a.V);
-  l.pg = plan(l.piece, a.N, a.D / 64, false);
-  l.px = plan(a.width, a.N, cdiv(l.piece, 64), true);
-  l.pw = plan(a.width, l.piece, cdiv(a.N, 64), true);
+  l.pg = plan(l.piece, a.N, a.D / 64);
+  // dx and dw run in one launch and share a tile form
+  double least = 1e30;
+  for (int f = 0; f < 3; ++f) {
+    const Plan x = plan_form(f, a.width, a.N, cdiv(l.piece, 64), true), w = plan_form(f, a.width, l.piece, cdiv(a.N, 64), true);
+    const double us = (need_x ? x.us : 0) + (need_w ? w.us : 0);
+    if (us < least) { least = us; l.px = x; l.pw = w; }
+  }
   l.bias_parts = cdiv(a.N, FORM_TILE[l.pg.form]) * FORM_WN[l.pg.form];
   l.dx_slab = l.px.splits > 1 || pieces > 1;
   const int64_t pvp = up(l.piece, 64);
@@ -529,14 +636,16 @@ bool sane(const DvXent& a) {
          ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0;
 }
 
-void launch_out(const DvXent& a, OutArgs g, const Plan& p, hipStream_t st) {
-  with_tile(p.form, [&](auto tile, auto b, auto, auto) {
+void launch_out(const DvXent& a, int form, const OutArgs& g0, const OutArgs& g1, const BiasArgs& bias, hipStream_t st) {
+  with_tile(form, [&](auto tile, auto b, auto, auto) {
     using T = decltype(tile);
     constexpr int B = decltype(b)::value;
-    const unsigned grid = (unsigned)(cdiv(g.M, B) * cdiv(g.N, B) * g.splits);
+    const int b0 = cdiv(g0.M, B) * cdiv(g0.N, B) * g0.splits, b1 = cdiv(g1.M, B) * cdiv(g1.N, B) * g1.splits;
+    const int b2 = bias.db ? cdiv(bias.pv, 64) : 0;
+    if (b0 + b1 + b2 == 0) return;
     static bool done[64];
     allow_lds(out_kernel<T, B, B>, T::LDS, done);
-    out_kernel<T, B, B><<<grid, T::NTHREADS, T::LDS, st>>>(a, g);
+    out_kernel<T, B, B><<<(unsigned)(b0 + b1 + b2), T::NTHREADS, T::LDS, st>>>(a, g0, g1, bias, b0, b1);
   });
 }
 void launch_reduce(const DvXent& a, const OutArgs& g, hipStream_t st) {
@@ -565,8 +674,11 @@ int dv_linear_xent_fwd(const DvXent& a, void* ws, float* lse, float* loss_rows, 
     allow_lds(stats_kernel<T, B, B, WM>, T::LDS, done);
     stats_kernel<T, B, B, WM><<<(unsigned)(cdiv(a.V, B) * cdiv(a.N, B)), T::NTHREADS, T::LDS, st>>>(a, part, psum, at_label);
   });
-  join_kernel<<<l.blocks, 1024, 0, st>>>(a, part, psum, at_label, l.parts, lse, loss_rows, blocks);
-  if (out) total_kernel<<<1, 256, 0, st>>>(blocks, l.blocks, a.reduction == DV_XENT_MEAN, out, total);
+  const int cols = FORM_TILE[l.p.form] / FORM_WM[l.p.form];
+  float2* lse2 = reinterpret_cast<float2*>(lse);
+  if (l.rows == 256) join_kernel<256><<<l.blocks, 1024, 0, st>>>(a, part, psum, at_label, l.parts, cols, lse2, loss_rows, blocks, out, total);
+  else join_kernel<64><<<l.blocks, 1024, 0, st>>>(a, part, psum, at_label, l.parts, cols, lse2, loss_rows, blocks, out, total);
+  if (out && l.blocks > 1) total_kernel<<<1, 256, 0, st>>>(blocks, l.blocks, a.reduction == DV_XENT_MEAN, out, total);
   return 0;
 }
 
@@ -579,42 +691,36 @@ int dv_linear_xent_bwd(const DvXent& a, void* ws, const float* lse, const void* 
   u16 *P = reinterpret_cast<u16*>(w + l.P), *Q = need_w ? reinterpret_cast<u16*>(w + l.Q) : nullptr;
   u16 *xt = reinterpret_cast<u16*>(w + l.xt), *wt = reinterpret_cast<u16*>(w + l.wt);
   float* pb = db ? reinterpret_cast<float*>(w + l.pb) : nullptr;
-  if (need_w) {
-    const dim3 grid((unsigned)(l.ldq / 64), (unsigned)cdiv(a.width, 64));
-    transpose_kernel<<<grid, 256, 0, st>>>(a, a.x, a.ldx, a.N, a.width, xt, l.ldq, 1);
-  }
+  auto transposed = [&](const u16* src, int64_t ld, int rows, u16* dst, int64_t ldd, int by_label) {
+    return Transpose{src, ld, rows, a.width, dst, ldd, by_label, (int)(ldd / 64) * cdiv(a.width, 64)};
+  };
   OutArgs gx{};
   for (int p0 = 0; p0 < a.V; p0 += l.piece) {
     const int pv = std::min(l.piece, a.V - p0), pvp = (int)up(pv, 64);
+    Transpose tx{}, tw{};
+    if (need_w && p0 == 0) tx = transposed(a.x, a.ldx, a.N, xt, l.ldq, 1);
+    if (need_x && !wt_all) tw = transposed(a.w + (int64_t)p0 * a.ldw, a.ldw, pv, wt, pvp, 0);
+    if (tx.blocks + tw.blocks) transpose_kernel<<<(unsigned)(tx.blocks + tw.blocks), 256, 0, st>>>(a, tx, tw);
     with_tile(l.pg.form, [&](auto tile, auto b, auto, auto wn) {
       using T = decltype(tile);
       constexpr int B = decltype(b)::value, WN = decltype(wn)::value;
       static bool done[64];
       allow_lds(grad_kernel<T, B, B, WN>, T::LDS, done);
-      grad_kernel<T, B, B, WN><<<(unsigned)(cdiv(pv, B) * cdiv(a.N, B)), T::NTHREADS, T::LDS, st>>>(a, lse, p0, pv, pvp, P, Q,
+      grad_kernel<T, B, B, WN><<<(unsigned)(cdiv(pv, B) * cdiv(a.N, B)), T::NTHREADS, T::LDS, st>>>(a, reinterpret_cast<const float2*>(lse), p0, pv, pvp, P, Q,
                                                                                                      l.ldq, pb);
     });
-    if (db) bias_kernel<<<cdiv(pv, 64), 256, 0, st>>>(a, pb, l.bias_parts, pv, db + p0, db_add);
-    if (need_x) {
-      const u16* wp = reinterpret_cast<const u16*>(wt_all) + p0;
-      int64_t ld = ldwt;
-      if (!wt_all) {
-        const dim3 grid((unsigned)(pvp / 64), (unsigned)cdiv(a.width, 64));
-        transpose_kernel<<<grid, 256, 0, st>>>(a, a.w + (int64_t)p0 * a.ldw, a.ldw, pv, a.width, wt, pvp, 0);
-        wp = wt;
-        ld = pvp;
-      }
-      gx = OutArgs{wp, P, ld, pvp, a.width, a.N, pvp / 64, std::min(l.px.splits, pvp / 64),
-                   l.dx_slab ? reinterpret_cast<float*>(w + l.sx) : nullptr, p0 > 0, dx, 0, 0, 1};
-      launch_out(a, gx, l.px, st);
-    }
+    OutArgs gw{};
+    if (need_x)
+      gx = OutArgs{wt_all ? reinterpret_cast<const u16*>(wt_all) + p0 : wt, P, wt_all ? ldwt : pvp, pvp, a.width, a.N, pvp / 64,
+                   std::min(l.px.splits, pvp / 64), l.dx_slab ? reinterpret_cast<float*>(w + l.sx) : nullptr, p0 > 0, dx, 0, 0, 1};
     if (need_w) {
       char* to = reinterpret_cast<char*>(dw) + (int64_t)p0 * a.width * (dw_f32 ? 4 : 2);
-      OutArgs gw{xt, Q, l.ldq, l.ldq, a.width, pv, (int)(l.ldq / 64), l.pw.splits,
-                 l.pw.splits > 1 ? reinterpret_cast<float*>(w + l.sw) : nullptr, 0, to, dw_f32, dw_add, 0};
-      launch_out(a, gw, l.pw, st);
-      if (l.pw.splits > 1) launch_reduce(a, gw, st);
+      gw = OutArgs{xt, Q, l.ldq, l.ldq, a.width, pv, (int)(l.ldq / 64), l.pw.splits,
+                   l.pw.splits > 1 ? reinterpret_cast<float*>(w + l.sw) : nullptr, 0, to, dw_f32, dw_add, 0};
     }
+    const BiasArgs gb{pb, l.bias_parts, pv, db ? db + p0 : nullptr, db_add};
+    launch_out(a, l.px.form, gx, gw, gb, st);
+    if (need_w && l.pw.splits > 1) launch_reduce(a, gw, st);
   }
   if (need_x && l.dx_slab) {
     gx.splits = l.px.splits;

@@ -154,7 +154,7 @@ def _linear_xent_forward(x, weight, bias, labels, smoothing, ignore_index, reduc
     args = (ptr(xk), xk.stride(0) if N > 1 else Dp, ptr(wk), wk.stride(0) if V > 1 else Dp, ptr(b), ptr(labels), N, V, Dp, D,
             *tail)
     ws = torch.empty(lib().linear_xent_fwd_bytes(*args), dtype=torch.uint8, device=dev)
-    lse = torch.empty(N, dtype=F32, device=dev) if train else None
+    lse = torch.empty((N, 2), dtype=F32, device=dev) if train else None
     rows = torch.empty(N, dtype=F32, device=dev) if reduction == 0 else None
     total = torch.empty(2, dtype=F32, device=dev) if reduction else None
     out = torch.empty((), dtype=F32, device=dev) if reduction else None

@@ -183,6 +183,12 @@ def test_wide_logits_and_classes_that_are_ruled_out():
     assert not grads[1][:512].any() and not grads[2][:512].any()
     b[:512] = torch.finfo(F32).min
     run_and_check(x, w, b, y)
+    b[:] = torch.finfo(F32).min  # every class: all logits round to the same value
+    loss = F.linear_cross_entropy(x, w, y, b, reduction="none")
+    torch.testing.assert_close(loss, torch.full_like(loss, torch.finfo(F32).min).sub(torch.finfo(F32).min).add(900.0).log())
+    wr = w.detach().clone().requires_grad_()
+    g = torch.autograd.grad(F.linear_cross_entropy(x, wr, y, b), wr)[0]
+    assert g.isfinite().all()
 
 
 @gpu
