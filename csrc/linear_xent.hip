@@ -29,6 +29,7 @@ namespace {
 using Big = GemmTile<256, 256, 2, 4>;
 using Mid = GemmTile<128, 128, 2, 2>;
 using Small = GemmTile<64, 64, 2, 2>;
+using Thin = ThinTile;
 
 constexpr int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 constexpr int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
@@ -96,6 +97,7 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void stats_kernel(D
   const int v0 = at.m * BM, n0 = at.n * BN;
   T t;
   t.run({a.w + (int64_t)v0 * a.ldw, a.ldw, a.V - v0}, {a.x + (int64_t)n0 * a.ldx, a.ldx, a.N - n0}, a.D / 64, smem);
+  if (!t.active()) return;
   add_bias<T, BM>(t, a, v0);
   const int vw = v0 + t.wm * T::TM * 32;  // the wave's columns: [vw, vw + 32 TM)
 #pragma unroll
@@ -150,11 +152,12 @@ __global__ __launch_bounds__(1024) void join_kernel(DvXent a, const float2* __re
                                                     float* __restrict__ total) {
   constexpr int STRIPS = 1024 / ROWS;
   __shared__ float sh[3][STRIPS][ROWS];
-  __shared__ float red[2][ROWS / 64];
+  __shared__ float red[2][ROWS < 64 ? 1 : ROWS / 64];
   const int j = threadIdx.x % ROWS, k = threadIdx.x / ROWS;
   const int64_t n = (int64_t)blockIdx.x * ROWS + j;
   float top = -INFINITY;
   if (n < a.N)
+#pragma unroll 8
     for (int p = k; p < parts; p += STRIPS) top = fmaxf(top, part[(int64_t)p * a.N + n].x);
   sh[0][k][j] = top;
   __syncthreads();
@@ -162,6 +165,7 @@ __global__ __launch_bounds__(1024) void join_kernel(DvXent a, const float2* __re
   for (int i = 0; i < STRIPS; ++i) top = fmaxf(top, sh[0][i][j]);
   float s = 0.f, sum = 0.f;  // of exp(l - top), of l - top
   if (n < a.N)
+#pragma unroll 8
     for (int p = k; p < parts; p += STRIPS) {
       const float2 q = part[(int64_t)p * a.N + n];
       s += q.x == -INFINITY ? q.y : q.y * exp2_fast((q.x - top) * LOG2E);  // (-inf: 0, or NaN)
@@ -191,12 +195,12 @@ __global__ __launch_bounds__(1024) void join_kernel(DvXent a, const float2* __re
   if (!out) return;
   l = wave_sum(l);
   one = wave_sum(one);
-  if (k == 0 && (j & 63) == 0) { red[0][j >> 6] = l; red[1][j >> 6] = one; }
+  if (threadIdx.x < (ROWS < 64 ? 64 : ROWS) && (threadIdx.x & 63) == 0) { red[0][threadIdx.x >> 6] = l; red[1][threadIdx.x >> 6] = one; }
   __syncthreads();
   if (threadIdx.x == 0) {
     l = one = 0.f;
 #pragma unroll
-    for (int i = 0; i < ROWS / 64; ++i) { l += red[0][i]; one += red[1][i]; }
+    for (int i = 0; i < (ROWS < 64 ? 1 : ROWS / 64); ++i) { l += red[0][i]; one += red[1][i]; }
     if (gridDim.x > 1) {
       blocks[blockIdx.x] = {l, one};
     } else {
@@ -233,11 +237,13 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(Dv
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int PITCH = 144;  // bytes: 64 bf16 + 16, conflict-free both ways
   constexpr int MG = T::TM < 2 ? 1 : 2, MW = 32 * MG, NW = 32 * T::TN;
-  const int tm = (pv + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
+  // tiles up to pvp and ldq: where a tile is half of 64 the last one may hold nothing but zeros of P or Q
+  const int tm = (pvp + BM - 1) / BM, tn = (int)((ldq + BN - 1) / BN);
   const TileAt at = tile_at(blockIdx.x, gridDim.x, tm, tn);
   const int v0 = at.m * BM, n0 = at.n * BN;  // v: within the piece
   T t;
-  t.run({a.w + (int64_t)(p0 + v0) * a.ldw, a.ldw, pv - v0}, {a.x + (int64_t)n0 * a.ldx, a.ldx, a.N - n0}, a.D / 64, smem);
+  t.run({a.w + (int64_t)(p0 + min(v0, pv - 1)) * a.ldw, a.ldw, max(pv - v0, 1)}, {a.x + (int64_t)min(n0, a.N - 1) * a.ldx, a.ldx, max(a.N - n0, 1)}, a.D / 64, smem);
+  if (!t.active()) return;
   add_bias<T, BM>(t, a, p0 + v0);
   const float off = a.smooth / a.V, hot = 1.f - a.smooth;
   const int vw0 = p0 + v0 + t.wm * T::TM * 32;
@@ -356,6 +362,7 @@ struct OutArgs {
 };
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 
 DV_DEVICE float out_scale(const DvXent& x, bool by_row, int64_t n, float common) {
   if (!by_row) return common;
@@ -419,6 +426,7 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void out_kernel(DvX
   T t;
   t.run({g.a + (int64_t)m0 * g.lda + k0 * 64, g.lda, g.M - m0}, {g.b + (int64_t)n0 * g.ldb + k0 * 64, g.ldb, g.N - n0},
         k1 - k0, smem);
+  if (!t.active()) return;
   const float common = g.slab ? 1.f : common_scale(x);
   char* mine = smem + t.wave * NW * PITCH;
 #pragma unroll
@@ -514,17 +522,28 @@ __global__ __launch_bounds__(256) void pack_kernel(const S* __restrict__ src, in
   for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < rows * (ldd / 8); u += (int64_t)gridDim.x * 256) {
     const int64_t r = u / (ldd / 8);
     const int c = (int)(u - r * (ldd / 8)) * 8;
-    uint32_t w[4];
+    const S* p = src + r * lds_ + c;
+    uint32_t w[4] = {};
+    if (c + 8 <= cols) {  // rows start at any element
+      if constexpr (sizeof(S) == 2) {
+        const u32x4_a2 q = *reinterpret_cast<const u32x4_a2*>(p);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float f[2];
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int i = c + 2 * e + k;
-        if constexpr (sizeof(S) == 2) f[k] = i < cols ? bf2f(src[r * lds_ + i]) : 0.f;
-        else f[k] = i < cols ? src[r * lds_ + i] : 0.f;
+        for (int e = 0; e < 4; ++e) w[e] = q[e];
+      } else {
+        const f32x4_a4 q0 = *reinterpret_cast<const f32x4_a4*>(p), q1 = *reinterpret_cast<const f32x4_a4*>(p + 4);
+        w[0] = pack2bf(q0[0], q0[1]); w[1] = pack2bf(q0[2], q0[3]);
+        w[2] = pack2bf(q1[0], q1[1]); w[3] = pack2bf(q1[2], q1[3]);
       }
-      w[e] = pack2bf(f[0], f[1]);
+    } else {
+      for (int e = 0; e < cols - c; ++e) {
+        uint32_t v;
+        if constexpr (sizeof(S) == 2) v = p[e];
+        else v = f2bf(p[e]);
+        const uint32_t at = v << (16 * (e & 1));
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k == e >> 1) w[k] |= at;
+      }
     }
     *reinterpret_cast<uint4*>(dst + r * ldd + c) = uint4{w[0], w[1], w[2], w[3]};
   }
@@ -534,35 +553,43 @@ __global__ __launch_bounds__(256) void pack_kernel(const S* __restrict__ src, in
 // Tile and split of an M x N x (64 ktiles) product: the least time by a model of one K-tile's time on
 // a full CU (throughput) and alone (latency), both measured.
 struct Plan { int form, splits; double us; };
-constexpr int FORM_TILE[3] = {256, 128, 64};
+constexpr int FORMS = 4, FORM_M[FORMS] = {256, 128, 64, 32}, FORM_N[FORMS] = {256, 128, 64, 32};
 Plan plan_form(int f, int64_t M, int64_t N, int ktiles, bool may_split) {
-  constexpr double FULL[3] = {1.6, 0.58, 0.25}, ALONE[3] = {1.6, 0.65, 0.35};  // us a K-tile
+  // us a K-tile: on a CU with as many blocks as fit (AT_ONCE), and alone; us of a block's two ends
+  constexpr double FULL[FORMS] = {1.6, 0.58, 0.25, 0.08}, ALONE[FORMS] = {1.6, 0.65, 0.35, 0.12}, ENDS[FORMS] = {4, 2.5, 2, 2.5};
+  constexpr int AT_ONCE[FORMS] = {1, 2, 5, 2};
   Plan best{f, 1, 1e30};
-  const int64_t tiles = (int64_t)cdiv(M, FORM_TILE[f]) * cdiv(N, FORM_TILE[f]);
+  const int64_t tiles = (int64_t)cdiv(M, FORM_M[f]) * cdiv(N, FORM_N[f]);
   for (int s = 1; s <= (may_split ? std::min(ktiles, 32) : 1); ++s) {
     const double k = cdiv(ktiles, s), blocks = (double)tiles * s;
     const double per_cu = f == 0 ? std::ceil(blocks / 256) : std::max(1.0, blocks / 256);
-    const double us = std::max(per_cu * k * FULL[f], k * ALONE[f]) + (s > 1 ? 4.0 + s * (double)M * N * 8 / 4e6 : 0.0);
+    const double rounds = std::ceil(blocks / (256 * AT_ONCE[f]));
+    const double us = ENDS[f] * rounds + std::max(per_cu * k * FULL[f], k * ALONE[f]) +
+                      (s > 1 ? 4.0 + s * (double)M * N * 8 / 4e6 : 0.0);
     if (us < best.us) best = {f, s, us};
   }
   return best;
 }
 Plan plan(int64_t M, int64_t N, int ktiles) {
   Plan best = plan_form(0, M, N, ktiles, false);
-  for (int f = 1; f < 3; ++f) {
+  for (int f = 1; f < FORMS; ++f) {
     const Plan p = plan_form(f, M, N, ktiles, false);
     if (p.us < best.us) best = p;
   }
   return best;
 }
 
+// f(tile, BM, BN, WM, WN)
+template <int V>
+using Int = std::integral_constant<int, V>;
 template <class F>
 void with_tile(int form, F&& f) {
-  if (form == 0) f(Big{}, std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
-  else if (form == 1) f(Mid{}, std::integral_constant<int, 128>{}, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
-  else f(Small{}, std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
+  if (form == 0) f(Big{}, Int<256>{}, Int<256>{}, Int<2>{}, Int<4>{});
+  else if (form == 1) f(Mid{}, Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{});
+  else if (form == 2) f(Small{}, Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{});
+  else f(Thin{}, Int<32>{}, Int<32>{}, Int<1>{}, Int<1>{});
 }
-constexpr int FORM_WM[3] = {2, 2, 2}, FORM_WN[3] = {4, 2, 2};
+constexpr int FORM_WM[FORMS] = {2, 2, 2, 1}, FORM_WN[FORMS] = {4, 2, 2, 1};
 
 // more than 64 KB of LDS, allowed once for each kernel and device
 template <class K>
@@ -578,8 +605,8 @@ struct FwdLayout { Plan p; int parts, rows, blocks; int64_t part, psum, label, b
 FwdLayout fwd_layout(const DvXent& a) {
   FwdLayout l;
   l.p = plan(a.V, a.N, a.D / 64);
-  l.parts = cdiv(a.V, FORM_TILE[l.p.form]) * FORM_WM[l.p.form];
-  l.rows = a.N <= 256 && l.parts <= 128 ? 256 : 64;  // small: one block joins every row
+  l.parts = cdiv(a.V, FORM_M[l.p.form]) * FORM_WM[l.p.form];
+  l.rows = a.N <= 256 && l.parts <= 128 ? 256 : 16;  // small: one block joins every row
   l.blocks = cdiv(a.N, l.rows);
   int64_t at = 0;
   auto take = [&](int64_t b) { const int64_t o = at; at += up(b, 256); return o; };
@@ -607,14 +634,14 @@ BwdLayout bwd_layout(const DvXent& a, bool need_x, bool need_w, bool need_b, boo
   const int pieces = cdiv(a.V, most);
   l.piece = (int)std::min<int64_t>(up(cdiv(a.V, pieces), 256), a.V);
   l.pg = plan(l.piece, a.N, a.D / 64);
-  // dx and dw run in one launch and share a tile form
+  // dx and dw run in one launch and share a tile form, whichever of them is wanted: a gradient's bits do
+  // not depend on which others are asked for
   double least = 1e30;
-  for (int f = 0; f < 3; ++f) {
+  for (int f = 0; f < FORMS; ++f) {
     const Plan x = plan_form(f, a.width, a.N, cdiv(l.piece, 64), true), w = plan_form(f, a.width, l.piece, cdiv(a.N, 64), true);
-    const double us = (need_x ? x.us : 0) + (need_w ? w.us : 0);
-    if (us < least) { least = us; l.px = x; l.pw = w; }
+    if (x.us + w.us < least) { least = x.us + w.us; l.px = x; l.pw = w; }
   }
-  l.bias_parts = cdiv(a.N, FORM_TILE[l.pg.form]) * FORM_WN[l.pg.form];
+  l.bias_parts = cdiv(l.ldq, FORM_N[l.pg.form]) * FORM_WN[l.pg.form];
   l.dx_slab = l.px.splits > 1 || pieces > 1;
   const int64_t pvp = up(l.piece, 64);
   int64_t at = 0;
@@ -637,15 +664,15 @@ bool sane(const DvXent& a) {
 }
 
 void launch_out(const DvXent& a, int form, const OutArgs& g0, const OutArgs& g1, const BiasArgs& bias, hipStream_t st) {
-  with_tile(form, [&](auto tile, auto b, auto, auto) {
+  with_tile(form, [&](auto tile, auto bm, auto bn, auto, auto) {
     using T = decltype(tile);
-    constexpr int B = decltype(b)::value;
-    const int b0 = cdiv(g0.M, B) * cdiv(g0.N, B) * g0.splits, b1 = cdiv(g1.M, B) * cdiv(g1.N, B) * g1.splits;
+    constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value;
+    const int b0 = cdiv(g0.M, BM) * cdiv(g0.N, BN) * g0.splits, b1 = cdiv(g1.M, BM) * cdiv(g1.N, BN) * g1.splits;
     const int b2 = bias.db ? cdiv(bias.pv, 64) : 0;
     if (b0 + b1 + b2 == 0) return;
     static bool done[64];
-    allow_lds(out_kernel<T, B, B>, T::LDS, done);
-    out_kernel<T, B, B><<<(unsigned)(b0 + b1 + b2), T::NTHREADS, T::LDS, st>>>(a, g0, g1, bias, b0, b1);
+    allow_lds(out_kernel<T, BM, BN>, T::LDS, done);
+    out_kernel<T, BM, BN><<<(unsigned)(b0 + b1 + b2), T::NTHREADS, T::LDS, st>>>(a, g0, g1, bias, b0, b1);
   });
 }
 void launch_reduce(const DvXent& a, const OutArgs& g, hipStream_t st) {
@@ -667,17 +694,17 @@ int dv_linear_xent_fwd(const DvXent& a, void* ws, float* lse, float* loss_rows, 
   float* psum = a.smooth > 0.f ? reinterpret_cast<float*>(w + l.psum) : nullptr;
   float* at_label = reinterpret_cast<float*>(w + l.label);
   float2* blocks = out ? reinterpret_cast<float2*>(w + l.block) : nullptr;
-  with_tile(l.p.form, [&](auto tile, auto b, auto wm, auto) {
+  with_tile(l.p.form, [&](auto tile, auto bm, auto bn, auto wm, auto) {
     using T = decltype(tile);
-    constexpr int B = decltype(b)::value, WM = decltype(wm)::value;
+    constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value;
     static bool done[64];
-    allow_lds(stats_kernel<T, B, B, WM>, T::LDS, done);
-    stats_kernel<T, B, B, WM><<<(unsigned)(cdiv(a.V, B) * cdiv(a.N, B)), T::NTHREADS, T::LDS, st>>>(a, part, psum, at_label);
+    allow_lds(stats_kernel<T, BM, BN, WM>, T::LDS, done);
+    stats_kernel<T, BM, BN, WM><<<(unsigned)(cdiv(a.V, BM) * cdiv(a.N, BN)), T::NTHREADS, T::LDS, st>>>(a, part, psum, at_label);
   });
-  const int cols = FORM_TILE[l.p.form] / FORM_WM[l.p.form];
+  const int cols = FORM_M[l.p.form] / FORM_WM[l.p.form];
   float2* lse2 = reinterpret_cast<float2*>(lse);
   if (l.rows == 256) join_kernel<256><<<l.blocks, 1024, 0, st>>>(a, part, psum, at_label, l.parts, cols, lse2, loss_rows, blocks, out, total);
-  else join_kernel<64><<<l.blocks, 1024, 0, st>>>(a, part, psum, at_label, l.parts, cols, lse2, loss_rows, blocks, out, total);
+  else join_kernel<16><<<l.blocks, 1024, 0, st>>>(a, part, psum, at_label, l.parts, cols, lse2, loss_rows, blocks, out, total);
   if (out && l.blocks > 1) total_kernel<<<1, 256, 0, st>>>(blocks, l.blocks, a.reduction == DV_XENT_MEAN, out, total);
   return 0;
 }
@@ -701,12 +728,12 @@ int dv_linear_xent_bwd(const DvXent& a, void* ws, const float* lse, const void* 
     if (need_w && p0 == 0) tx = transposed(a.x, a.ldx, a.N, xt, l.ldq, 1);
     if (need_x && !wt_all) tw = transposed(a.w + (int64_t)p0 * a.ldw, a.ldw, pv, wt, pvp, 0);
     if (tx.blocks + tw.blocks) transpose_kernel<<<(unsigned)(tx.blocks + tw.blocks), 256, 0, st>>>(a, tx, tw);
-    with_tile(l.pg.form, [&](auto tile, auto b, auto, auto wn) {
+    with_tile(l.pg.form, [&](auto tile, auto bm, auto bn, auto, auto wn) {
       using T = decltype(tile);
-      constexpr int B = decltype(b)::value, WN = decltype(wn)::value;
+      constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WN = decltype(wn)::value;
       static bool done[64];
-      allow_lds(grad_kernel<T, B, B, WN>, T::LDS, done);
-      grad_kernel<T, B, B, WN><<<(unsigned)(cdiv(pv, B) * cdiv(a.N, B)), T::NTHREADS, T::LDS, st>>>(a, reinterpret_cast<const float2*>(lse), p0, pv, pvp, P, Q,
+      allow_lds(grad_kernel<T, BM, BN, WN>, T::LDS, done);
+      grad_kernel<T, BM, BN, WN><<<(unsigned)(cdiv(pvp, BM) * cdiv(l.ldq, BN)), T::NTHREADS, T::LDS, st>>>(a, reinterpret_cast<const float2*>(lse), p0, pv, pvp, P, Q,
                                                                                                      l.ldq, pb);
     });
     OutArgs gw{};

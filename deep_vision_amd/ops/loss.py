@@ -90,44 +90,6 @@ def _cached_weight(weight):
     return weight.dtype == F32 and isinstance(weight, torch.nn.Parameter) and weight.is_contiguous()
 
 
-class _LinearXentFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, labels, smoothing, ignore_index, reduction):
-        with on_device(x):
-            track_leaves(ctx, x, weight, bias)
-            loss, ctx.cfg, saved = _linear_xent_forward(x, weight, bias, labels, smoothing, ignore_index, reduction, True)
-        ctx.save_for_backward(x, weight, bias, *saved)
-        return loss
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, go):
-        x, weight, bias, labels, xk, wk, b, lse, total = ctx.saved_tensors
-        N, V, D, tail = ctx.cfg  # D: padded to whole K-tiles
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dev = x.device
-        sw = accumulation_sink(ctx, 1, weight) if need_w else None
-        sb = accumulation_sink(ctx, 2, bias) if need_b else None
-        dx = torch.empty((N, x.shape[1]), dtype=BF16, device=dev) if need_x else None
-        dw = sw if sw is not None else torch.empty(weight.shape, dtype=weight.dtype, device=dev) if need_w else None
-        db = sb if sb is not None else torch.empty(V, dtype=F32, device=dev) if need_b else None
-        go = go.detach().to(F32).reshape(-1).contiguous()
-        with on_device(x):
-            wt, Vp = None, (V + 63) // 64 * 64
-            if wk is None:
-                wk = _operand(weight, D)
-                if need_x and Vp <= 1 << 22:
-                    wt = _transposed_operand(weight, Vp)
-            args = (ptr(xk), xk.stride(0) if N > 1 else D, ptr(wk), wk.stride(0) if V > 1 else D, ptr(b), ptr(labels), N, V,
-                    D, x.shape[1], *tail)
-            nbytes = lib().linear_xent_bwd_bytes(*args, int(need_x), int(need_w), int(need_b), int(wt is not None))
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-            lib().linear_xent_bwd(*args, ptr(go), ptr(total), ptr(ws), ptr(lse), ptr(wt), Vp, ptr(dx),
-                                  ptr(dw), int(weight.dtype == F32), int(sw is not None), ptr(db), int(sb is not None),
-                                  stream_handle())
-        return dx, None if sw is not None else dw, None if sb is not None else db, None, None, None, None
-
-
 def _operand(weight, Dp):
     from .conv import _prep_weight
 
@@ -143,24 +105,72 @@ def _transposed_operand(weight, Vp):
 
 
 def _linear_xent_forward(x, weight, bias, labels, smoothing, ignore_index, reduction, train):
+    """(loss, what backward needs beside x and weight, the native calls' shared arguments)."""
     N, D = x.shape
     V, dev = weight.shape[0], x.device
     Dp = (D + 63) // 64 * 64
-    xk = _bf16_rows(x.detach(), D, Dp)
+    xk = _bf16_rows(x, D, Dp)
     cached = _cached_weight(weight)
-    wk = _operand(weight, Dp) if cached else _bf16_rows(weight.detach(), D, Dp)
-    b = bias.detach().contiguous() if bias is not None else None
-    tail = (ignore_index, smoothing, reduction)
+    wk = _operand(weight, Dp) if cached else _bf16_rows(weight, D, Dp)
+    b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     args = (ptr(xk), xk.stride(0) if N > 1 else Dp, ptr(wk), wk.stride(0) if V > 1 else Dp, ptr(b), ptr(labels), N, V, Dp, D,
-            *tail)
+            ignore_index, smoothing, reduction)
     ws = torch.empty(lib().linear_xent_fwd_bytes(*args), dtype=torch.uint8, device=dev)
-    lse = torch.empty((N, 2), dtype=F32, device=dev) if train else None
-    rows = torch.empty(N, dtype=F32, device=dev) if reduction == 0 else None
-    total = torch.empty(2, dtype=F32, device=dev) if reduction else None
-    out = torch.empty((), dtype=F32, device=dev) if reduction else None
-    lib().linear_xent_fwd(*args, ptr(ws), ptr(lse), ptr(rows), ptr(total), ptr(out), stream_handle())
-    saved = (labels, xk, None if cached else wk, b, lse, total)
-    return (out if reduction else rows), (N, V, Dp, tail), saved
+    # per row (largest logit, log2 of the sum above it); behind them (sum of the losses, rows that count)
+    stats = torch.empty(2 * N + 2, dtype=F32, device=dev)
+    loss = torch.empty(() if reduction else N, dtype=F32, device=dev)
+    at = stats.data_ptr()
+    if reduction:
+        lib().linear_xent_fwd(*args, ptr(ws), at if train else 0, 0, at + 8 * N, ptr(loss), stream_handle())
+    else:
+        lib().linear_xent_fwd(*args, ptr(ws), at if train else 0, ptr(loss), 0, 0, stream_handle())
+    return loss, (labels, xk, None if cached else wk, b, stats), args
+
+
+class _LinearXentFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, labels, smoothing, ignore_index, reduction):
+        with on_device(x):
+            track_leaves(ctx, x, weight, bias)
+            loss, saved, ctx.args = _linear_xent_forward(x, weight, bias, labels, smoothing, ignore_index, reduction, True)
+        ctx.save_for_backward(x, weight, bias, *saved)
+        return loss
+
+    @staticmethod
+    def backward(ctx, go):
+        if torch.is_grad_enabled():
+            return _linear_xent_once(ctx, go)
+        return _linear_xent_backward(ctx, go)
+
+
+def _linear_xent_backward(ctx, go):
+    x, weight, bias, labels, xk, wk, b, stats = ctx.saved_tensors  # labels .. stats hold what ctx.args points to
+    N, V, Dp = ctx.args[6:9]
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    dev = x.device
+    sw = accumulation_sink(ctx, 1, weight) if need_w else None
+    sb = accumulation_sink(ctx, 2, bias) if need_b else None
+    dx = torch.empty((N, x.shape[1]), dtype=BF16, device=dev) if need_x else None
+    dw = sw if sw is not None else torch.empty(weight.shape, dtype=weight.dtype, device=dev) if need_w else None
+    db = sb if sb is not None else torch.empty(V, dtype=F32, device=dev) if need_b else None
+    if go.dtype != F32 or not go.is_contiguous():
+        go = go.to(F32).contiguous()
+    with on_device(x):
+        args, wt, Vp = ctx.args, None, (V + 63) // 64 * 64
+        if wk is None:  # the parameter's cached operands, as they are now
+            wk = _operand(weight, Dp)
+            args = (*args[:2], ptr(wk), *args[3:])
+            if need_x and Vp <= 1 << 22:
+                wt = _transposed_operand(weight, Vp)
+        ws = torch.empty(lib().linear_xent_bwd_bytes(*args, int(need_x), int(need_w), int(need_b), int(wt is not None)),
+                         dtype=torch.uint8, device=dev)
+        at = stats.data_ptr()
+        lib().linear_xent_bwd(*args, ptr(go), at + 8 * N, ptr(ws), at, ptr(wt), Vp, ptr(dx), ptr(dw),
+                              int(weight.dtype == F32), int(sw is not None), ptr(db), int(sb is not None), stream_handle())
+    return dx, None if sw is not None else dw, None if sb is not None else db, None, None, None, None
+
+
+_linear_xent_once = torch.autograd.function.once_differentiable(_linear_xent_backward)  # no second derivative
 
 
 def linear_cross_entropy(x, weight, labels, bias=None, label_smoothing=0.0, ignore_index=-100, reduction="mean"):
@@ -188,7 +198,10 @@ def linear_cross_entropy(x, weight, labels, bias=None, label_smoothing=0.0, igno
         raise ValueError(f"linear_cross_entropy: label_smoothing must lie in [0, 1], got {label_smoothing}")
     same_device("linear_cross_entropy", x, weight, labels, bias)
     D = x.shape[-1]
-    x2, flat = x.reshape(-1, D), labels.reshape(-1).long()
+    x2 = x if x.dim() == 2 else x.reshape(-1, D)
+    flat = labels if labels.dim() == 1 else labels.reshape(-1)
+    if flat.dtype != torch.int64:
+        flat = flat.long()
     for name, t, kinds in (("x", x, (BF16, F32)), ("weight", weight, (BF16, F32)), ("bias", bias, (F32,))):
         if t is not None and t.dtype not in kinds and native(x):
             raise TypeError(f"linear_cross_entropy: {name} must be {' or '.join(str(k)[6:] for k in kinds)}, got {t.dtype}")
@@ -202,7 +215,7 @@ def linear_cross_entropy(x, weight, labels, bias=None, label_smoothing=0.0, igno
     code = _REDUCTIONS[reduction]
     if x2.dtype != BF16:
         x2 = x2.to(BF16)
-    args = (x2, weight, bias, flat.contiguous(), float(label_smoothing), int(ignore_index), code)
+    args = (x2, weight, bias, flat if flat.is_contiguous() else flat.contiguous(), float(label_smoothing), int(ignore_index), code)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, weight, bias)):
         loss = _LinearXentFn.apply(*args)
     else:
