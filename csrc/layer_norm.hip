@@ -109,8 +109,10 @@ DV_DEVICE void load_param(const float* w, int c, int D, float fill, float (&v)[E
 // sums of a and b over the LANES lanes of a row; LANES > 64 means the whole block
 template <int LANES>
 DV_DEVICE void row_sum2(float& a, float& b, float (*sh)[2]) {
+  a = row16_sum(a);  // 16 lanes by DPP, the rest through LDS
+  b = row16_sum(b);
 #pragma unroll
-  for (int o = (LANES < 64 ? LANES : 64) / 2; o > 0; o >>= 1) {
+  for (int o = 16; o < (LANES < 64 ? LANES : 64); o <<= 1) {
     a += __shfl_xor(a, o, 64);
     b += __shfl_xor(b, o, 64);
   }
@@ -249,8 +251,8 @@ __global__ __launch_bounds__(bwd_block_of(LANES)) void ln_bwd_kernel(const T* __
       }
     }
     row_sum2<LANES>(s, q, sh);
-    s *= inv;
-    q *= inv;
+    s *= inv * rstd;
+    q *= inv * rstd * rstd;
     if (dx) {
 #pragma unroll
       for (int k = 0; k < VECS; ++k) {
@@ -261,7 +263,7 @@ __global__ __launch_bounds__(bwd_block_of(LANES)) void ln_bwd_kernel(const T* __
         Vec<T>::unpack(cg[k], g);
         weight(k, wv);
 #pragma unroll
-        for (int e = 0; e < E; ++e) g[e] = (g[e] * wv[e] - s - (v[e] - mu) * rstd * q) * rstd;
+        for (int e = 0; e < E; ++e) g[e] = g[e] * (wv[e] * rstd) - ((v[e] - mu) * q + s);
         store_cols<T, TAIL>(dx + r * D, (lane + k * LANES) * E, D, g);
       }
     }
@@ -466,7 +468,7 @@ int dv_layer_norm_parts(int is_bf16, int64_t rows, int D) {
   auto form = [&](auto l, auto k, auto) {
     constexpr int L = decltype(l)::value;
     per = bwd_block_of(L) / L;
-    most = L < 64 ? 1536 : L == 64 ? (decltype(k)::value == 1 ? 512 : 256) : L == 256 ? 512 : 256;
+    most = L < 64 ? 1280 : L == 64 ? (decltype(k)::value == 1 ? 512 : 256) : L == 256 ? 512 : 256;
   };
   const bool held = is_bf16 ? with_form<u16>(D, form) : with_form<float>(D, form);
   if (!held) return (int)std::min<int64_t>(rows, 64);

@@ -91,31 +91,37 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     """y = (x - mean) / sqrt(var + eps) * weight + bias over the last ``len(normalized_shape)``
     dimensions of ``x``. On the GPU ``x`` is bf16 or fp32, ``weight`` and ``bias`` fp32 (or None);
     y has x's type. ``eps`` > 0."""
-    shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(int(n) for n in normalized_shape)
-    if not shape or tuple(x.shape[-len(shape):]) != shape or len(shape) > x.dim():
+    shape = (normalized_shape,) if isinstance(normalized_shape, int) else tuple(normalized_shape)
+    lead = x.dim() - len(shape)
+    if not shape or lead < 0 or x.shape[lead:] != shape:
         raise ValueError(f"layer_norm: the last dimensions of an input of shape {tuple(x.shape)} are not {shape}")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and tuple(t.shape) != shape:
-            raise ValueError(f"layer_norm: {name} has shape {tuple(t.shape)}, expected {shape}")
-    if not eps > 0 or not math.isfinite(eps):
+    if not 0 < eps < math.inf:
         raise ValueError(f"layer_norm: eps must be positive and finite, got {eps}")
+    on_gpu = native(x)
+    train = torch.is_grad_enabled() and x.requires_grad
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if t.shape != shape:
+            raise ValueError(f"layer_norm: {name} has shape {tuple(t.shape)}, expected {shape}")
+        if on_gpu and t.dtype != F32:
+            raise TypeError(f"layer_norm: {name} must be float32, got {t.dtype}")
+        train = train or (t.requires_grad and torch.is_grad_enabled())
     same_device("layer_norm", x, weight, bias)
-    if not native(x):
+    if not on_gpu:
         w, b = (t.to(x.dtype) if t is not None and x.dtype == torch.float64 else t for t in (weight, bias))
         wide = TF.layer_norm(x if x.dtype == torch.float64 else x.float(), shape, w, b, eps)
         return wide.to(x.dtype)
-    if x.dtype not in (BF16, F32):
+    if x.dtype != BF16 and x.dtype != F32:
         raise TypeError(f"layer_norm: the input must be bfloat16 or float32, got {x.dtype}")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and t.dtype != F32:
-            raise TypeError(f"layer_norm: {name} must be float32, got {t.dtype}")
-    D = math.prod(shape)
+    D = shape[0] if len(shape) == 1 else math.prod(shape)
     if D == 0:
         raise ValueError("layer_norm: a normalized dimension is empty")
-    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias))):
+    if not train:
         with on_device(x):
-            x2, ld = _rows(x.detach(), D)
-            return _forward(x2, ld, _dense(weight), _dense(bias), float(eps), False)[0].view(x.shape)
+            x2, ld = _rows(x, D)
+            y = _forward(x2, ld, _dense(weight), _dense(bias), float(eps), False)[0]
+        return y if x.dim() == 2 and lead == 1 else y.view(x.shape)
     if len(shape) > 1:
         x2 = x.reshape(*x.shape[:-len(shape)], D)
         weight, bias = (t.reshape(D) if t is not None else None for t in (weight, bias))

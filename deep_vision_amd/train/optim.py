@@ -102,6 +102,7 @@ class _FlatOptimizer(torch.optim.Optimizer):
             for p, (off, _) in zip(ps, offs):
                 p._dv_off = off
         f = dict(param=pflat, grad=gflat, views=views, gviews=gviews, offsets=offs, step=0, first=True, shared=shared)
+        f["ptrs"] = [v.data_ptr() for v in views]
         f["states"] = self._new_states(f)
         if old is not None:  # re-bound after the parameters moved: carry the optimizer state over
             f["step"], f["first"] = old["step"], old["first"]
@@ -138,9 +139,8 @@ class _FlatOptimizer(torch.optim.Optimizer):
         for gi, (group, f) in enumerate(zip(self.param_groups, self._flat)):
             if f is None:
                 continue
-            shared = f["shared"]
-            if all(getattr(p, "_dv_flat", None) is shared and p.data_ptr() == v.data_ptr()
-                   for p, v in zip(group["params"], f["views"])):
+            # (the buffer this optimizer holds stays allocated: a parameter moved elsewhere has another address)
+            if [p.data_ptr() for p in group["params"]] == f["ptrs"]:
                 continue
             if f["param"].is_cuda and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("parameters were re-flattened under a graph capture")
@@ -258,6 +258,8 @@ class _FlatOptimizer(torch.optim.Optimizer):
 
     def _sync_grads(self, group, f):
         """Ensure every .grad is the flat view; returns active (offset, n) segments."""
+        if all([p.grad is gv for p, gv in zip(group["params"], f["gviews"])]):
+            return [(0, f["param"].numel())]
         segs = []
         all_active = True
         for p, gv, (off, n) in zip(group["params"], f["gviews"], f["offsets"]):
@@ -560,20 +562,21 @@ class FusedAdamW(_FlatOptimizer):
             return
         b1, b2 = g["betas"]
         _, bc1, bc2 = self._hparams(g, f["step"])
-        p, gr, s = f["param"][off:off + n], f["grad"][off:off + n], f["states"]
-        if p.is_cuda:
-            args = (float(g["lr"]), float(b1), float(b2), float(g["eps"]), float(g["weight_decay"]), float(bc1), float(bc2),
-                    float(gs))
-            with on_device(p):
+        s = f["states"]
+        if f["param"].is_cuda:
+            args = (float(g["lr"]), float(b1), float(b2), float(g["eps"]), float(g["weight_decay"]), bc1, bc2, float(gs))
+            at, gat = ptr(f["param"]), ptr(f["grad"])
+            with on_device(f["param"]):
                 if self.state_bits == 32:
-                    lib().adamw32(ptr(p), ptr(gr), ptr(s["exp_avg"][off:off + n]), ptr(s["exp_avg_sq"][off:off + n]), n,
+                    lib().adamw32(at + 4 * off, gat + 4 * off, ptr(s["exp_avg"]) + 4 * off, ptr(s["exp_avg_sq"]) + 4 * off, n,
                                   *args, self._hp_ptr(f), self._skip_ptr(), stream_handle())
                     return
                 lo, hi = bisect_left(f["chunk_starts"], off), bisect_left(f["chunk_starts"], off + n)
-                lib().adamw8(ptr(f["param"]), ptr(f["grad"]), ptr(s["exp_avg"]), ptr(s["exp_avg_scale"]),
-                             ptr(s["exp_avg_root"]), ptr(s["exp_avg_root_scale"]), ptr(f["chunks"][lo:hi]), hi - lo, *args,
+                lib().adamw8(at, gat, ptr(s["exp_avg"]), ptr(s["exp_avg_scale"]), ptr(s["exp_avg_root"]),
+                             ptr(s["exp_avg_root_scale"]), ptr(f["chunks"]) + 24 * lo, hi - lo, *args,
                              f["step"] & 0xFFFFFFFF, self.seed, self._hp_ptr(f), self._skip_ptr(), stream_handle())
             return
+        p, gr = f["param"][off:off + n], f["grad"][off:off + n]
         if self.state_bits == 32:
             self._update_cpu(g, p, gr * gs, s["exp_avg"][off:off + n], s["exp_avg_sq"][off:off + n], bc1, bc2)
             return
