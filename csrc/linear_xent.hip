@@ -554,9 +554,11 @@ __global__ __launch_bounds__(256) void pack_kernel(const S* __restrict__ src, in
 // a full CU (throughput) and alone (latency), both measured.
 struct Plan { int form, splits; double us; };
 constexpr int FORMS = 4, FORM_M[FORMS] = {256, 128, 64, 32}, FORM_N[FORMS] = {256, 128, 64, 32};
-Plan plan_form(int f, int64_t M, int64_t N, int ktiles, bool may_split) {
+enum Ends { PLAIN, GRAD };  // what a block does behind its sums: GRAD writes both layouts of d
+Plan plan_form(int f, int64_t M, int64_t N, int ktiles, bool may_split, Ends ends) {
   // us a K-tile: on a CU with as many blocks as fit (AT_ONCE), and alone; us of a block's two ends
-  constexpr double FULL[FORMS] = {1.6, 0.58, 0.25, 0.08}, ALONE[FORMS] = {1.6, 0.65, 0.35, 0.12}, ENDS[FORMS] = {4, 2.5, 2, 2.5};
+  constexpr double FULL[FORMS] = {1.6, 0.58, 0.25, 0.2}, ALONE[FORMS] = {1.6, 0.65, 0.35, 0.2};
+  constexpr double ENDS[2][FORMS] = {{4, 2.5, 2, 2.5}, {16, 9, 4, 5}};
   constexpr int AT_ONCE[FORMS] = {1, 2, 5, 2};
   Plan best{f, 1, 1e30};
   const int64_t tiles = (int64_t)cdiv(M, FORM_M[f]) * cdiv(N, FORM_N[f]);
@@ -564,16 +566,16 @@ Plan plan_form(int f, int64_t M, int64_t N, int ktiles, bool may_split) {
     const double k = cdiv(ktiles, s), blocks = (double)tiles * s;
     const double per_cu = f == 0 ? std::ceil(blocks / 256) : std::max(1.0, blocks / 256);
     const double rounds = std::ceil(blocks / (256 * AT_ONCE[f]));
-    const double us = ENDS[f] * rounds + std::max(per_cu * k * FULL[f], k * ALONE[f]) +
+    const double us = ENDS[ends][f] * rounds + std::max(per_cu * k * FULL[f], k * ALONE[f]) +
                       (s > 1 ? 4.0 + s * (double)M * N * 8 / 4e6 : 0.0);
     if (us < best.us) best = {f, s, us};
   }
   return best;
 }
-Plan plan(int64_t M, int64_t N, int ktiles) {
-  Plan best = plan_form(0, M, N, ktiles, false);
+Plan plan(int64_t M, int64_t N, int ktiles, Ends ends) {
+  Plan best = plan_form(0, M, N, ktiles, false, ends);
   for (int f = 1; f < FORMS; ++f) {
-    const Plan p = plan_form(f, M, N, ktiles, false);
+    const Plan p = plan_form(f, M, N, ktiles, false, ends);
     if (p.us < best.us) best = p;
   }
   return best;
@@ -604,7 +606,7 @@ void allow_lds(K kernel, int bytes, bool (&done)[64]) {
 struct FwdLayout { Plan p; int parts, rows, blocks; int64_t part, psum, label, block, bytes; };
 FwdLayout fwd_layout(const DvXent& a) {
   FwdLayout l;
-  l.p = plan(a.V, a.N, a.D / 64);
+  l.p = plan(a.V, a.N, a.D / 64, PLAIN);
   l.parts = cdiv(a.V, FORM_M[l.p.form]) * FORM_WM[l.p.form];
   l.rows = a.N <= 256 && l.parts <= 128 ? 256 : 16;  // small: one block joins every row
   l.blocks = cdiv(a.N, l.rows);
@@ -633,12 +635,13 @@ BwdLayout bwd_layout(const DvXent& a, bool need_x, bool need_w, bool need_b, boo
   const int64_t most = std::max<int64_t>(PIECE_BYTES / (4 * l.ldq) / 256 * 256, 256);
   const int pieces = cdiv(a.V, most);
   l.piece = (int)std::min<int64_t>(up(cdiv(a.V, pieces), 256), a.V);
-  l.pg = plan(l.piece, a.N, a.D / 64);
+  l.pg = plan(l.piece, a.N, a.D / 64, GRAD);
   // dx and dw run in one launch and share a tile form, whichever of them is wanted: a gradient's bits do
   // not depend on which others are asked for
   double least = 1e30;
   for (int f = 0; f < FORMS; ++f) {
-    const Plan x = plan_form(f, a.width, a.N, cdiv(l.piece, 64), true), w = plan_form(f, a.width, l.piece, cdiv(a.N, 64), true);
+    const Plan x = plan_form(f, a.width, a.N, cdiv(l.piece, 64), true, PLAIN),
+               w = plan_form(f, a.width, l.piece, cdiv(a.N, 64), true, PLAIN);
     if (x.us + w.us < least) { least = x.us + w.us; l.px = x; l.pw = w; }
   }
   l.bias_parts = cdiv(l.ldq, FORM_N[l.pg.form]) * FORM_WN[l.pg.form];

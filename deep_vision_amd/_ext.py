@@ -59,5 +59,10 @@ def stream_handle(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def current_device() -> int:
+    """Index of the current HIP device (of an initialised process: the raw query)."""
+    return torch.cuda.current_device() if _CUR_DEV is None else _CUR_DEV()
+
+
 def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()

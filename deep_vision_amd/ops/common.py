@@ -14,7 +14,7 @@ import weakref
 
 import torch
 
-from .._ext import lib, ptr, stream_handle  # noqa: F401
+from .._ext import current_device, lib, ptr, stream_handle  # noqa: F401
 
 BF16 = torch.bfloat16
 F32 = torch.float32
@@ -181,8 +181,8 @@ def grad_sink(param):
 
 
 def accumulation_sink(ctx, index, param):
-    """``grad_sink(param)`` where this backward pass is going to add the gradient of input ``index``
-    to ``param.grad``; None under ``torch.autograd.grad`` (which wants the gradient returned and
+    """``grad_sink(param)`` where this backward pass is going to add the gradient of the ``index``-th
+    tensor among the function's inputs (None is not one) to ``param.grad``; None under ``torch.autograd.grad`` (which wants the gradient returned and
     ``.grad`` untouched), for a pass that leaves the parameter out, and where the parameter has
     hooks that read its gradient."""
     sink = grad_sink(param)
@@ -231,7 +231,7 @@ class on_device:
 
     def __init__(self, x):
         i = x.device.index
-        self.guard = None if i is None or i == torch.cuda.current_device() else torch.cuda.device(i)
+        self.guard = None if i is None or i == current_device() else torch.cuda.device(i)
 
     def __enter__(self):
         if self.guard is not None:

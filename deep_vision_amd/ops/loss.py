@@ -104,8 +104,14 @@ def _transposed_operand(weight, Vp):
     return _prep_weight(weight.view(V, D, 1, 1), 1, Vp, mode=1, param=weight)
 
 
+def _linear_xent_args(xk, wk, b, labels, V, Dp, D, ignore_index, smoothing, reduction):
+    N = xk.shape[0]
+    return (ptr(xk), xk.stride(0) if N > 1 else Dp, ptr(wk), wk.stride(0) if V > 1 else Dp, ptr(b), ptr(labels), N, V, Dp, D,
+            ignore_index, smoothing, reduction)
+
+
 def _linear_xent_forward(x, weight, bias, labels, smoothing, ignore_index, reduction, train):
-    """(loss, what backward needs beside x and weight, the native calls' shared arguments)."""
+    """(loss, what backward needs beside x and weight)."""
     N, D = x.shape
     V, dev = weight.shape[0], x.device
     Dp = (D + 63) // 64 * 64
@@ -113,8 +119,7 @@ def _linear_xent_forward(x, weight, bias, labels, smoothing, ignore_index, reduc
     cached = _cached_weight(weight)
     wk = _operand(weight, Dp) if cached else _bf16_rows(weight, D, Dp)
     b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    args = (ptr(xk), xk.stride(0) if N > 1 else Dp, ptr(wk), wk.stride(0) if V > 1 else Dp, ptr(b), ptr(labels), N, V, Dp, D,
-            ignore_index, smoothing, reduction)
+    args = _linear_xent_args(xk, wk, b, labels, V, Dp, D, ignore_index, smoothing, reduction)
     ws = torch.empty(lib().linear_xent_fwd_bytes(*args), dtype=torch.uint8, device=dev)
     # per row (largest logit, log2 of the sum above it); behind them (sum of the losses, rows that count)
     stats = torch.empty(2 * N + 2, dtype=F32, device=dev)
@@ -124,7 +129,7 @@ def _linear_xent_forward(x, weight, bias, labels, smoothing, ignore_index, reduc
         lib().linear_xent_fwd(*args, ptr(ws), at if train else 0, 0, at + 8 * N, ptr(loss), stream_handle())
     else:
         lib().linear_xent_fwd(*args, ptr(ws), at if train else 0, ptr(loss), 0, 0, stream_handle())
-    return loss, (labels, xk, None if cached else wk, b, stats), args
+    return loss, (labels, xk, None if cached else wk, b, stats)
 
 
 class _LinearXentFn(torch.autograd.Function):
@@ -132,7 +137,8 @@ class _LinearXentFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, labels, smoothing, ignore_index, reduction):
         with on_device(x):
             track_leaves(ctx, x, weight, bias)
-            loss, saved, ctx.args = _linear_xent_forward(x, weight, bias, labels, smoothing, ignore_index, reduction, True)
+            loss, saved = _linear_xent_forward(x, weight, bias, labels, smoothing, ignore_index, reduction, True)
+        ctx.cfg = (smoothing, ignore_index, reduction)
         ctx.save_for_backward(x, weight, bias, *saved)
         return loss
 
@@ -144,29 +150,31 @@ class _LinearXentFn(torch.autograd.Function):
 
 
 def _linear_xent_backward(ctx, go):
-    x, weight, bias, labels, xk, wk, b, stats = ctx.saved_tensors  # labels .. stats hold what ctx.args points to
-    N, V, Dp = ctx.args[6:9]
+    x, weight, bias, labels, xk, wk, b, stats = ctx.saved_tensors
+    smoothing, ignore_index, reduction = ctx.cfg
+    N, D = x.shape
+    V, Dp = weight.shape[0], (D + 63) // 64 * 64
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
     dev = x.device
     sw = accumulation_sink(ctx, 1, weight) if need_w else None
     sb = accumulation_sink(ctx, 2, bias) if need_b else None
-    dx = torch.empty((N, x.shape[1]), dtype=BF16, device=dev) if need_x else None
+    dx = torch.empty((N, D), dtype=BF16, device=dev) if need_x else None
     dw = sw if sw is not None else torch.empty(weight.shape, dtype=weight.dtype, device=dev) if need_w else None
     db = sb if sb is not None else torch.empty(V, dtype=F32, device=dev) if need_b else None
     if go.dtype != F32 or not go.is_contiguous():
         go = go.to(F32).contiguous()
-    with on_device(x):
-        args, wt, Vp = ctx.args, None, (V + 63) // 64 * 64
-        if wk is None:  # the parameter's cached operands, as they are now
-            wk = _operand(weight, Dp)
-            args = (*args[:2], ptr(wk), *args[3:])
-            if need_x and Vp <= 1 << 22:
-                wt = _transposed_operand(weight, Vp)
-        ws = torch.empty(lib().linear_xent_bwd_bytes(*args, int(need_x), int(need_w), int(need_b), int(wt is not None)),
-                         dtype=torch.uint8, device=dev)
-        at = stats.data_ptr()
-        lib().linear_xent_bwd(*args, ptr(go), at + 8 * N, ptr(ws), at, ptr(wt), Vp, ptr(dx), ptr(dw),
-                              int(weight.dtype == F32), int(sw is not None), ptr(db), int(sb is not None), stream_handle())
+    # (the engine runs a node on the device and stream of its forward pass)
+    wt, Vp = None, (V + 63) // 64 * 64
+    if wk is None:  # the parameter's cached operands, as they are now
+        wk = _operand(weight, Dp)
+        if need_x and Vp <= 1 << 22:
+            wt = _transposed_operand(weight, Vp)
+    args = _linear_xent_args(xk, wk, b, labels, V, Dp, D, ignore_index, smoothing, reduction)
+    ws = torch.empty(lib().linear_xent_bwd_bytes(*args, int(need_x), int(need_w), int(need_b), int(wt is not None)),
+                     dtype=torch.uint8, device=dev)
+    at = stats.data_ptr()
+    lib().linear_xent_bwd(*args, ptr(go), at + 8 * N, ptr(ws), at, ptr(wt), Vp, ptr(dx), ptr(dw),
+                          int(weight.dtype == F32), int(sw is not None), ptr(db), int(sb is not None), stream_handle())
     return dx, None if sw is not None else dw, None if sb is not None else db, None, None, None, None
 
 

@@ -72,15 +72,15 @@ def _backward(ctx, dy):
         return dx, torch.zeros_like(weight) if need_w else None, torch.zeros_like(bias) if need_b else None, None
     g, ldg = _rows(dy if dy.dtype == dtype else dy.to(dtype), D)
     sw = accumulation_sink(ctx, 1, weight) if need_w else None
-    sb = accumulation_sink(ctx, 2, bias) if need_b else None
+    sb = accumulation_sink(ctx, 1 if weight is None else 2, bias) if need_b else None
     dw = sw if sw is not None else torch.empty(D, dtype=F32, device=dev) if need_w else None
     db = sb if sb is not None else torch.empty(D, dtype=F32, device=dev) if need_b else None
     bf16 = int(dtype == BF16)
     parts = lib().layer_norm_parts(bf16, rows, D)
     part = torch.empty(parts * 2 * D, dtype=F32, device=dev) if need_w or need_b else None
-    with on_device(x):
-        lib().layer_norm_bwd(ptr(x), bf16, ctx.ld, ptr(g), ldg, ptr(w), ptr(stats), ptr(dx), ptr(part), parts, ptr(dw), ptr(db),
-                             int(sw is not None), int(sb is not None), rows, D, stream_handle())
+    # (the engine runs a node on the device and stream of its forward pass)
+    lib().layer_norm_bwd(ptr(x), bf16, ctx.ld, ptr(g), ldg, ptr(w), ptr(stats), ptr(dx), ptr(part), parts, ptr(dw), ptr(db),
+                         int(sw is not None), int(sb is not None), rows, D, stream_handle())
     return dx, None if sw is not None else dw, None if sb is not None else db, None
 
 

@@ -137,9 +137,10 @@ def test_8_bit_step_and_rounding(dev):
         g = torch.zeros_like(m0)
         g[:n] = p.grad.double()
         m, v = 0.9 * m0 + 0.1 * g, 0.999 * r0 * r0 + 0.001 * g * g
-        move = KW["lr"] / (1 - 0.9 ** 4) * m / (v.sqrt() / math.sqrt(1 - 0.999 ** 4) + KW["eps"])
+        per = KW["lr"] / (1 - 0.9 ** 4) / (v.sqrt() / math.sqrt(1 - 0.999 ** 4) + KW["eps"])
+        move, terms = per * m, per * (0.9 * m0.abs() + 0.1 * g.abs())  # m's products round whatever cancels
         want = q * (1 - KW["lr"] * KW["weight_decay"]) - move[:n]
-        assert ((p.detach().double() - want).abs() <= 3 * U * want.abs() + 24 * U * move[:n].abs()).all()
+        assert ((p.detach().double() - want).abs() <= 3 * U * want.abs() + 24 * U * terms[:n]).all()
         for name, t in (("exp_avg", m), ("exp_avg_root", v.sqrt())):
             got, _ = wide(new, name, at, n)
             top = t.abs().view(e, 256).amax(1, keepdim=True).expand(e, 256).reshape(-1)
@@ -345,3 +346,27 @@ def test_two_groups_and_another_stream(bits):
         torch.cuda.current_stream().wait_stream(s)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
     assert len(one.flat_params()) == len(one.flat_states()) == 2
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_past_32_bits_of_values(bits):
+    """2^31 zeros before a tensor (which stay: no gradient, no moments, no decay of zero): the tensor
+    behind them moves as it does alone, its noise apart (another place)."""
+    tail = tensors([5000], DEV)[0]
+    big = torch.nn.Parameter(torch.zeros((1 << 31) + 13, device=DEV))
+    far, near = torch.nn.Parameter(tail.clone()), torch.nn.Parameter(tail.clone())
+    one = FusedAdamW([big, far], **KW, state_bits=bits)
+    two = FusedAdamW([near], **KW, state_bits=bits)
+    for step in range(2):
+        feed([near], step)
+        far.grad.copy_(near.grad)
+        one.step()
+        two.step()
+        if bits == 32 or step == 0:
+            assert torch.equal(far, near)
+    assert not big[:1000].any() and not big[-1000:].any()
+    a, b = one.state_dict()["state"][1], two.state_dict()["state"][0]
+    for k in a:
+        if k.endswith("_scale") or bits == 32:
+            torch.testing.assert_close(a[k], b[k], rtol=0.3 if bits == 8 else 0, atol=0)

@@ -258,6 +258,10 @@ def test_gradients_accumulate_into_a_live_buffer():
     m(x).backward(dy)
     assert m.weight.grad is buf
     assert torch.equal(m.weight.grad, gw + 2) and torch.equal(m.bias.grad, gb - 1)
+    only = torch.full_like(b, 0.5).requires_grad_()  # a bias without a weight
+    only.grad = torch.ones_like(only)
+    F.layer_norm(x, 200, None, only).backward(dy)
+    assert torch.equal(only.grad, gb + 1)
     again = torch.autograd.grad(m(x), (m.weight, m.bias), dy)  # leaves .grad alone
     assert torch.equal(again[0], gw) and torch.equal(again[1], gb) and torch.equal(m.weight.grad, gw + 2)
     y = m(x)
