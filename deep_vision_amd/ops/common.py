@@ -194,6 +194,29 @@ def accumulation_sink(ctx, index, param):
         return None
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, what, grad, *leaves):
+        ctx.what = what
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, *unused):
+        raise RuntimeError(f"{ctx.what} has no second derivative (create_graph=True)")
+
+
+def first_derivative_only(what, backward, ctx, go):
+    """``backward(ctx, go, sinks)`` of an op without a second derivative. Under create_graph=True the
+    gradients depend on everything the op did, and differentiating them raises: torch's
+    once_differentiable lets them pass as constants where ``go`` itself needs no gradient."""
+    if not torch.is_grad_enabled():
+        return backward(ctx, go, True)
+    inputs = [t for t in (go, *ctx.saved_tensors) if t is not None and t.requires_grad]
+    with torch.no_grad():
+        grads = backward(ctx, go, False)
+    return tuple(g if g is None or not inputs else _NoSecondDerivative.apply(what, g, *inputs) for g in grads)
+
+
 _GRAPHS = {}  # id(leaf) -> [(weak reference to an autograd node that uses it, the node's stream)]
 
 

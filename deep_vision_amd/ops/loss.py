@@ -8,8 +8,8 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as TF
 
-from .common import (BF16, F32, accumulation_sink, lib, native, on_device, ptr, same_device, stream_handle,
-                     track_leaves)
+from .common import (BF16, F32, accumulation_sink, first_derivative_only, lib, native, on_device, ptr, same_device,
+                     stream_handle, track_leaves)
 
 
 class _XentFn(torch.autograd.Function):
@@ -144,20 +144,18 @@ class _LinearXentFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, go):
-        if torch.is_grad_enabled():
-            return _linear_xent_once(ctx, go)
-        return _linear_xent_backward(ctx, go)
+        return first_derivative_only("linear_cross_entropy", _linear_xent_backward, ctx, go)
 
 
-def _linear_xent_backward(ctx, go):
+def _linear_xent_backward(ctx, go, sinks):
     x, weight, bias, labels, xk, wk, b, stats = ctx.saved_tensors
     smoothing, ignore_index, reduction = ctx.cfg
     N, D = x.shape
     V, Dp = weight.shape[0], (D + 63) // 64 * 64
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
     dev = x.device
-    sw = accumulation_sink(ctx, 1, weight) if need_w else None
-    sb = accumulation_sink(ctx, 2, bias) if need_b else None
+    sw = accumulation_sink(ctx, 1, weight) if need_w and sinks else None
+    sb = accumulation_sink(ctx, 2, bias) if need_b and sinks else None
     dx = torch.empty((N, D), dtype=BF16, device=dev) if need_x else None
     dw = sw if sw is not None else torch.empty(weight.shape, dtype=weight.dtype, device=dev) if need_w else None
     db = sb if sb is not None else torch.empty(V, dtype=F32, device=dev) if need_b else None
@@ -176,9 +174,6 @@ def _linear_xent_backward(ctx, go):
     lib().linear_xent_bwd(*args, ptr(go), at + 8 * N, ptr(ws), at, ptr(wt), Vp, ptr(dx), ptr(dw),
                           int(weight.dtype == F32), int(sw is not None), ptr(db), int(sb is not None), stream_handle())
     return dx, None if sw is not None else dw, None if sb is not None else db, None, None, None, None
-
-
-_linear_xent_once = torch.autograd.function.once_differentiable(_linear_xent_backward)  # no second derivative
 
 
 def linear_cross_entropy(x, weight, labels, bias=None, label_smoothing=0.0, ignore_index=-100, reduction="mean"):

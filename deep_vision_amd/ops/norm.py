@@ -12,7 +12,8 @@ import math
 import torch
 import torch.nn.functional as TF
 
-from .common import BF16, F32, accumulation_sink, lib, native, on_device, ptr, same_device, stream_handle, track_leaves
+from .common import (BF16, F32, accumulation_sink, first_derivative_only, lib, native, on_device, ptr, same_device,
+                     stream_handle, track_leaves)
 
 
 def _rows(t, D):
@@ -47,23 +48,20 @@ class _LayerNormFn(torch.autograd.Function):
     def forward(ctx, x, weight, bias, eps):
         with on_device(x):
             track_leaves(ctx, x, weight, bias)
-            x2, ctx.ld = _rows(x, x.shape[-1])
-            w = _dense(weight)
-            y, stats = _forward(x2, ctx.ld, w, _dense(bias), eps, True)
-        ctx.save_for_backward(x2, w, stats)
-        ctx.params = (weight, bias)  # leaves whose gradient may go straight into a live .grad
+            x2, ld = _rows(x, x.shape[-1])
+            y, stats = _forward(x2, ld, _dense(weight), _dense(bias), eps, True)
+        ctx.save_for_backward(x, weight, bias, stats)
         return y if x.dim() == 2 else y.view(x.shape)
 
     @staticmethod
     def backward(ctx, dy):
-        if torch.is_grad_enabled():
-            return _once(ctx, dy)
-        return _backward(ctx, dy)
+        return first_derivative_only("layer_norm", _backward, ctx, dy)
 
 
-def _backward(ctx, dy):
-    x, w, stats = ctx.saved_tensors
-    weight, bias = ctx.params
+def _backward(ctx, dy, sinks):
+    x, weight, bias, stats = ctx.saved_tensors
+    x, ld = _rows(x, x.shape[-1])
+    w = _dense(weight)
     rows, D = x.shape
     dev, dtype = x.device, x.dtype
     need_x, need_w, need_b, _ = ctx.needs_input_grad
@@ -71,20 +69,17 @@ def _backward(ctx, dy):
     if not rows:
         return dx, torch.zeros_like(weight) if need_w else None, torch.zeros_like(bias) if need_b else None, None
     g, ldg = _rows(dy if dy.dtype == dtype else dy.to(dtype), D)
-    sw = accumulation_sink(ctx, 1, weight) if need_w else None
-    sb = accumulation_sink(ctx, 1 if weight is None else 2, bias) if need_b else None
+    sw = accumulation_sink(ctx, 1, weight) if need_w and sinks else None
+    sb = accumulation_sink(ctx, 1 if weight is None else 2, bias) if need_b and sinks else None
     dw = sw if sw is not None else torch.empty(D, dtype=F32, device=dev) if need_w else None
     db = sb if sb is not None else torch.empty(D, dtype=F32, device=dev) if need_b else None
     bf16 = int(dtype == BF16)
     parts = lib().layer_norm_parts(bf16, rows, D)
     part = torch.empty(parts * 2 * D, dtype=F32, device=dev) if need_w or need_b else None
     # (the engine runs a node on the device and stream of its forward pass)
-    lib().layer_norm_bwd(ptr(x), bf16, ctx.ld, ptr(g), ldg, ptr(w), ptr(stats), ptr(dx), ptr(part), parts, ptr(dw), ptr(db),
+    lib().layer_norm_bwd(ptr(x), bf16, ld, ptr(g), ldg, ptr(w), ptr(stats), ptr(dx), ptr(part), parts, ptr(dw), ptr(db),
                          int(sw is not None), int(sb is not None), rows, D, stream_handle())
     return dx, None if sw is not None else dw, None if sb is not None else db, None
-
-
-_once = torch.autograd.function.once_differentiable(_backward)  # create_graph=True: no second derivative
 
 
 def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):

@@ -270,6 +270,30 @@ def test_gradients_accumulate_into_a_live_buffer():
 
 
 @gpu
+def test_saved_tensors_kept_elsewhere_and_recomputation():
+    from torch.utils.checkpoint import checkpoint
+
+    wide, w, b, dy = make(21, 300, torch.bfloat16)
+    x = wide[:, 4:204].detach().requires_grad_()  # strided: what comes back from the host is not
+    w, b, dy = w[:200].clone().requires_grad_(), b[:200].clone().requires_grad_(), dy[:, :200]
+    want = torch.autograd.grad(F.layer_norm(x, 200, w, b), (x, w, b), dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = F.layer_norm(x, 200, w, b)
+    got = torch.autograd.grad(y, (x, w, b), dy)
+    again = torch.autograd.grad(checkpoint(lambda t: F.layer_norm(t, 200, w, b), x, use_reentrant=False), (x, w, b), dy)
+    assert all(torch.equal(p, q) and torch.equal(p, r) for p, q, r in zip(want, got, again))
+
+
+@gpu
+def test_no_second_derivative():
+    x, w, b, dy = make(4, 32, torch.float32)
+    x.requires_grad_()
+    g = torch.autograd.grad(F.layer_norm(x, 32, w, b), x, dy, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        g.sum().backward()
+
+
+@gpu
 def test_another_stream_and_a_replayed_graph():
     x, w, b, dy = make(300, 512, torch.bfloat16)
     x.requires_grad_()

@@ -354,6 +354,53 @@ def test_some_gradients_only_and_a_retained_graph():
 
 
 @gpu
+def test_saved_tensors_kept_elsewhere_and_recomputation():
+    from torch.utils.checkpoint import checkpoint
+
+    wide, w, b, y = make(50, 200, 300)
+    for x in (wide[:, :128], wide[:, 3:103]):  # used in place, and packed
+        x = x.detach().requires_grad_()
+        wx, bx = w[:, :x.shape[1]].detach().clone().requires_grad_(), b.clone().requires_grad_()
+        want = torch.autograd.grad(F.linear_cross_entropy(x, wx, y, bx), (x, wx, bx))
+        with torch.autograd.graph.save_on_cpu():
+            loss = F.linear_cross_entropy(x, wx, y, bx)
+        got = torch.autograd.grad(loss, (x, wx, bx))
+        again = torch.autograd.grad(checkpoint(lambda t: F.linear_cross_entropy(t, wx, y, bx), x, use_reentrant=False),
+                                    (x, wx, bx))
+        assert all(torch.equal(p, q) and torch.equal(p, r) for p, q, r in zip(want, got, again))
+
+
+@gpu
+def test_what_changes_between_the_passes_is_refused():
+    x, w, b, y = make(20, 64, 90)
+    w.requires_grad_()
+    loss = F.linear_cross_entropy(x, w, y, b)
+    y[0] += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    loss = F.linear_cross_entropy(x, w, y, b)
+    g = torch.autograd.grad(loss, w, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        g.sum().backward()
+
+
+@gpu
+def test_shared_weight_and_broadcast_rows():
+    """One weight as classifier twice and in an elementwise term, one row broadcast to a batch: autograd
+    adds what each use gives (sums of bf16 gradients: h of the largest partial sum each)."""
+    x, w, b, y = make(40, 128, 200)
+    row = x[:1].detach().clone().requires_grad_()
+    w = w.requires_grad_()
+    one = torch.autograd.grad(F.linear_cross_entropy(row.expand(40, 128), w, y, b), (row, w))
+    two = torch.autograd.grad(F.linear_cross_entropy(x, w, y, b), w)[0]
+    loss = F.linear_cross_entropy(row.expand(40, 128), w, y, b) + F.linear_cross_entropy(x, w, y, b) + w.float().sum()
+    got = torch.autograd.grad(loss, (row, w))
+    assert torch.equal(got[0], one[0])
+    want = one[1].double() + two.double() + 1
+    assert ((got[1].double() - want).abs() <= 2 * H * (one[1].double().abs() + two.double().abs() + 1)).all()
+
+
+@gpu
 def test_two_streams_and_a_replayed_graph():
     x, w, b, y = make(512, 256, 3000, ignored=0.1)
     want = run_and_check(x, w, b, y)
