@@ -385,6 +385,7 @@ PYBIND11_MODULE(_C, m) {
 #undef XENT
 #undef XENT_ARGS
   m.attr("XENT_MAX_ROWS") = DV_XENT_MAX_ROWS;
+  m.attr("XENT_MAX_CLASSES") = DV_XENT_MAX_CLASSES;
   m.def("pack_rows", [](uptr src, int bf16, int64_t lds, int64_t rows, int cols, uptr dst, int64_t ldd, uptr st) {
     if (dv_pack_rows(CP(src), bf16, lds, rows, cols, P(dst), ldd, ST(st))) throw std::runtime_error("pack_rows: unsupported shape");
     check_last("pack_rows");

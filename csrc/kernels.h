@@ -260,7 +260,7 @@ int dv_adamw8(const DvAdamW& a, const void* chunks, int nchunks, float* p, const
 
 // ---- linear + softmax cross entropy (linear_xent.hip) ----
 enum { DV_XENT_NONE = 0, DV_XENT_MEAN = 1, DV_XENT_SUM = 2 };
-constexpr int DV_XENT_MAX_ROWS = 1 << 22;
+constexpr int DV_XENT_MAX_ROWS = 1 << 22, DV_XENT_MAX_CLASSES = 1 << 30;
 struct DvXent {
   const uint16_t *x, *w;   // bf16 [N][ldx], [V][ldw]: D columns, zeros from `width` on
   int64_t ldx, ldw;

@@ -142,8 +142,8 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void stats_kernel(D
 }
 
 // ROWS rows a block, 1024 / ROWS strips of the parts: (largest logit, log2 of the sum of exponentials
-// above it) of each row, kept apart so that a large common offset costs no precision, and its loss; the block's (sum, count),
-// or where one block holds every row the result itself
+// above it) of each row, kept apart so that a large common offset costs no precision, and its loss; the
+// block's (sum, count), or where one block holds every row the result itself
 template <int ROWS>
 __global__ __launch_bounds__(1024) void join_kernel(DvXent a, const float2* __restrict__ part, const float* __restrict__ psum,
                                                     const float* __restrict__ at_label, int parts, int cols_a_part,
@@ -195,7 +195,10 @@ __global__ __launch_bounds__(1024) void join_kernel(DvXent a, const float2* __re
   if (!out) return;
   l = wave_sum(l);
   one = wave_sum(one);
-  if (threadIdx.x < (ROWS < 64 ? 64 : ROWS) && (threadIdx.x & 63) == 0) { red[0][threadIdx.x >> 6] = l; red[1][threadIdx.x >> 6] = one; }
+  if (threadIdx.x < (ROWS < 64 ? 64 : ROWS) && (threadIdx.x & 63) == 0) {
+    red[0][threadIdx.x >> 6] = l;
+    red[1][threadIdx.x >> 6] = one;
+  }
   __syncthreads();
   if (threadIdx.x == 0) {
     l = one = 0.f;
@@ -227,7 +230,7 @@ __global__ __launch_bounds__(256) void total_kernel(const float2* __restrict__ b
 }
 
 // --------------------------------------------------------------------------------------- backward
-// d of the piece [p0, p0 + pv) of the vocabulary: P [n][ldp], zero up to pvp columns, and
+// d of the piece [p0, p0 + pv) of the vocabulary: P [n][pvp], zero from pv on, and
 // Q = t . d [v][ldq], zero up to ldq; db partial sums [n block and wave][pv]
 template <class T, int BM, int BN, int WN>
 __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(DvXent a, const float2* __restrict__ lse, int p0,
@@ -242,7 +245,8 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(Dv
   const TileAt at = tile_at(blockIdx.x, gridDim.x, tm, tn);
   const int v0 = at.m * BM, n0 = at.n * BN;  // v: within the piece
   T t;
-  t.run({a.w + (int64_t)(p0 + min(v0, pv - 1)) * a.ldw, a.ldw, max(pv - v0, 1)}, {a.x + (int64_t)min(n0, a.N - 1) * a.ldx, a.ldx, max(a.N - n0, 1)}, a.D / 64, smem);
+  t.run({a.w + (int64_t)(p0 + min(v0, pv - 1)) * a.ldw, a.ldw, max(pv - v0, 1)},
+        {a.x + (int64_t)min(n0, a.N - 1) * a.ldx, a.ldx, max(a.N - n0, 1)}, a.D / 64, smem);
   if (!t.active()) return;
   add_bias<T, BM>(t, a, p0 + v0);
   const float off = a.smooth / a.V, hot = 1.f - a.smooth;
@@ -663,7 +667,8 @@ BwdLayout bwd_layout(const DvXent& a, bool need_x, bool need_w, bool need_b, boo
 }
 
 bool sane(const DvXent& a) {
-  return a.N > 0 && a.N <= DV_XENT_MAX_ROWS && a.V > 0 && a.D > 0 && a.D % 64 == 0 && a.width > 0 && a.width <= a.D &&
+  return a.N > 0 && a.N <= DV_XENT_MAX_ROWS && a.V > 0 && a.V <= DV_XENT_MAX_CLASSES &&
+         (int64_t)cdiv(a.V, 32) * cdiv(a.N, 32) < 0x7fffffff && a.D > 0 && a.D % 64 == 0 && a.width > 0 && a.width <= a.D &&
          a.ldx >= a.D && a.ldw >= a.D && a.ldx % 8 == 0 && a.ldw % 8 == 0 && a.ldx <= (1 << 22) && a.ldw <= (1 << 22) &&
          ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0;
 }

@@ -217,7 +217,7 @@ def first_derivative_only(what, backward, ctx, go):
     return tuple(g if g is None or not inputs else _NoSecondDerivative.apply(what, g, *inputs) for g in grads)
 
 
-_GRAPHS = {}  # id(leaf) -> [(weak reference to an autograd node that uses it, the node's stream)]
+_GRAPHS = {}  # id(leaf) -> [(weak references to an autograd node that uses it and to the leaf, the node's stream)]
 
 
 def track_leaves(ctx, *leaves):
@@ -230,11 +230,11 @@ def track_leaves(ctx, *leaves):
     for t in leaves:
         if t is None or not t.requires_grad or not t.is_leaf:
             continue
-        alive = [e for e in _GRAPHS.get(id(t), ()) if e[0]() is not None]
-        if capturing and any(s != stream for _, s in alive):
+        alive = [e for e in _GRAPHS.get(id(t), ()) if e[0]() is not None and e[1]() is t]
+        if capturing and any(e[2] != stream for e in alive):
             raise RuntimeError("an eager autograd graph of this tensor is still alive (a loss or output that holds it): "
                                "delete it before capturing a backward pass over the same tensor")
-        alive.append((me, stream))
+        alive.append((me, weakref.ref(t), stream))
         _GRAPHS[id(t)] = alive
     if len(_GRAPHS) > 4096:
         for k in [k for k, v in _GRAPHS.items() if all(e[0]() is None for e in v)]:

@@ -186,7 +186,8 @@ def linear_cross_entropy(x, weight, labels, bias=None, label_smoothing=0.0, igno
     whatever x holds there. ``reduction`` is "mean" over the rows that count (0 if none does), "sum",
     or "none" (labels' shape). Products are summed in fp32, the loss and bias gradient are fp32, the
     gradient of the logits is rounded to bf16 for the two products behind it; the weight's gradient
-    has the weight's type and goes straight into a live ``.grad`` buffer. At most 2^22 rows."""
+    has the weight's type and goes straight into a live ``.grad`` buffer. At most 2^22 rows and 2^30
+    classes."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
@@ -213,6 +214,9 @@ def linear_cross_entropy(x, weight, labels, bias=None, label_smoothing=0.0, igno
         return loss.reshape(labels.shape) if reduction == "none" else loss
     if x2.shape[0] > int(lib().XENT_MAX_ROWS):
         raise ValueError(f"linear_cross_entropy: {x2.shape[0]} rows, at most {int(lib().XENT_MAX_ROWS)} in a call")
+    V = weight.shape[0]
+    if V > int(lib().XENT_MAX_CLASSES) or (V // 32 + 1) * (x2.shape[0] // 32 + 1) >= 1 << 31:
+        raise ValueError(f"linear_cross_entropy: {x2.shape[0]} rows against {V} classes are more than a call takes")
     if D > 1 << 22:
         raise ValueError(f"linear_cross_entropy: rows of {D} values, at most {1 << 22}")
     code = _REDUCTIONS[reduction]
