@@ -13,8 +13,8 @@
 //  * backward, for each piece of the vocabulary: the product again, its epilogue writes d in bf16 both
 //    ways round ([n][v] and [v][n]), because each of the two products that follow wants its own sum
 //    index contiguous; then dx += d w and dw = d' x. x' and the piece of w' are laid out once a call.
-//  * d is rounded to bf16 before it is scaled: (p - 1) is then exact to half a step whatever the batch
-//    size, and the scale is applied to the fp32 sums. Only with an upstream gradient for each row
+//  * d is rounded to bf16 before it is scaled (and divided by 1 - e): a label's entry p - 1 then rounds the
+//    same whatever the batch size, and the scale is applied to the fp32 sums. Only with an upstream gradient for each row
 //    does d' carry it (the sum over n cannot).
 //  * a row whose label is ignored (or lies outside [0, V)) takes no part: its d is zero and so is its
 //    row of x', whatever x holds there.
@@ -51,9 +51,13 @@ DV_DEVICE void wave_sync() {
 }
 
 DV_DEVICE bool counted(int64_t label, const DvXent& a) { return label != a.ignore && label >= 0 && label < a.V; }
+// d is held divided by this, so that a label's entry is -1 plus a probability and rounds to a step of 1: all
+// entries at -0.9 would round the same way
+DV_DEVICE float unit(const DvXent& a) { return a.smooth < 1.f ? 1.f - a.smooth : 1.f; }
 // the factor of every row's gradient that does not depend on the row
 DV_DEVICE float common_scale(const DvXent& a) {
-  return a.reduction == DV_XENT_NONE ? 1.f : a.reduction == DV_XENT_SUM ? a.go[0] : a.go[0] / fmaxf(a.total[1], 1.f);
+  const float s = a.reduction == DV_XENT_NONE ? 1.f : a.reduction == DV_XENT_SUM ? a.go[0] : a.go[0] / fmaxf(a.total[1], 1.f);
+  return s * unit(a);
 }
 
 // exp(a - b) as exp2((a - b) * LOG2E): subtracted first, since a class ruled out by the type's lowest
@@ -249,7 +253,7 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(Dv
         {a.x + (int64_t)min(n0, a.N - 1) * a.ldx, a.ldx, max(a.N - n0, 1)}, a.D / 64, smem);
   if (!t.active()) return;
   add_bias<T, BM>(t, a, p0 + v0);
-  const float off = a.smooth / a.V, hot = 1.f - a.smooth;
+  const float inv = 1.f / unit(a), off = a.smooth / a.V * inv, hot = a.smooth < 1.f ? 1.f : 0.f;
   const int vw0 = p0 + v0 + t.wm * T::TM * 32;
   float ts[T::TN];
 #pragma unroll
@@ -262,7 +266,7 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(Dv
 #pragma unroll
     for (int i = 0; i < T::TM; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) t.acc[i][j][r] = exp2_fast(fmaf(t.acc[i][j][r] - z.x, LOG2E, -z.y)) - off;
+      for (int r = 0; r < 16; ++r) t.acc[i][j][r] = fmaf(exp2_fast(fmaf(t.acc[i][j][r] - z.x, LOG2E, -z.y)), inv, -off);
     const bool here = use && label >= vw0 && label < vw0 + T::TM * 32;
     if (__any(here)) {
       const int rel = here ? (int)label - vw0 - 4 * (t.lane >> 5) : -1;
@@ -371,7 +375,7 @@ typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 DV_DEVICE float out_scale(const DvXent& x, bool by_row, int64_t n, float common) {
   if (!by_row) return common;
   if (!counted(x.labels[n], x)) return 0.f;
-  return x.reduction == DV_XENT_NONE ? x.go[n] : common;
+  return x.reduction == DV_XENT_NONE ? x.go[n] * common : common;
 }
 DV_DEVICE void put4(void* out, int f32, int add, int64_t o, int left, f32x4 v) {
   if (f32) {
