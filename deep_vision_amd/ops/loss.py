@@ -8,7 +8,7 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as TF
 
-from .common import (BF16, F32, accumulation_sink, first_derivative_only, lib, native, on_device, ptr, same_device,
+from .common import (BF16, F32, accumulation_sink, fast_apply, first_derivative_only, lib, native, on_device, ptr, same_device,
                      stream_handle, track_leaves)
 
 
@@ -153,12 +153,11 @@ def _linear_xent_backward(ctx, go, sinks):
     N, D = x.shape
     V, Dp = weight.shape[0], (D + 63) // 64 * 64
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
-    dev = x.device
     sw = accumulation_sink(ctx, 1, weight) if need_w and sinks else None
     sb = accumulation_sink(ctx, 2, bias) if need_b and sinks else None
-    dx = torch.empty((N, D), dtype=BF16, device=dev) if need_x else None
-    dw = sw if sw is not None else torch.empty(weight.shape, dtype=weight.dtype, device=dev) if need_w else None
-    db = sb if sb is not None else torch.empty(V, dtype=F32, device=dev) if need_b else None
+    dx = x.new_empty((N, D)) if need_x else None
+    dw = sw if sw is not None else weight.new_empty((V, D)) if need_w else None
+    db = sb if sb is not None else bias.new_empty(V) if need_b else None
     if go.dtype != F32 or not go.is_contiguous():
         go = go.to(F32).contiguous()
     # (the engine runs a node on the device and stream of its forward pass)
@@ -168,12 +167,15 @@ def _linear_xent_backward(ctx, go, sinks):
         if need_x and Vp <= 1 << 22:
             wt = _transposed_operand(weight, Vp)
     args = _linear_xent_args(xk, wk, b, labels, V, Dp, D, ignore_index, smoothing, reduction)
-    ws = torch.empty(lib().linear_xent_bwd_bytes(*args, int(need_x), int(need_w), int(need_b), int(wt is not None)),
-                     dtype=torch.uint8, device=dev)
+    ws = x.new_empty(lib().linear_xent_bwd_bytes(*args, int(need_x), int(need_w), int(need_b), int(wt is not None)),
+                     dtype=torch.uint8)
     at = stats.data_ptr()
     lib().linear_xent_bwd(*args, ptr(go), at + 8 * N, ptr(ws), at, ptr(wt), Vp, ptr(dx), ptr(dw),
                           int(weight.dtype == F32), int(sw is not None), ptr(db), int(sb is not None), stream_handle())
     return dx, None if sw is not None else dw, None if sb is not None else db, None, None, None, None
+
+
+_apply_linear_xent = fast_apply(_LinearXentFn)
 
 
 def linear_cross_entropy(x, weight, labels, bias=None, label_smoothing=0.0, ignore_index=-100, reduction="mean"):
@@ -224,7 +226,7 @@ def linear_cross_entropy(x, weight, labels, bias=None, label_smoothing=0.0, igno
         x2 = x2.to(BF16)
     args = (x2, weight, bias, flat if flat.is_contiguous() else flat.contiguous(), float(label_smoothing), int(ignore_index), code)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, weight, bias)):
-        loss = _LinearXentFn.apply(*args)
+        loss = _apply_linear_xent(*args)
     else:
         with on_device(x):
             loss = _linear_xent_forward(x2, weight, bias, *args[3:], False)[0]

@@ -12,7 +12,7 @@ import math
 import torch
 import torch.nn.functional as TF
 
-from .common import (BF16, F32, accumulation_sink, first_derivative_only, lib, native, on_device, ptr, same_device,
+from .common import (BF16, F32, accumulation_sink, fast_apply, first_derivative_only, lib, native, on_device, ptr, same_device,
                      stream_handle, track_leaves)
 
 
@@ -59,27 +59,31 @@ class _LayerNormFn(torch.autograd.Function):
 
 
 def _backward(ctx, dy, sinks):
+    # runs on autograd's device thread, where every Python step costs more than in the forward pass
     x, weight, bias, stats = ctx.saved_tensors
-    x, ld = _rows(x, x.shape[-1])
-    w = _dense(weight)
-    rows, D = x.shape
-    dev, dtype = x.device, x.dtype
     need_x, need_w, need_b, _ = ctx.needs_input_grad
-    dx = torch.empty(dy.shape, dtype=dtype, device=dev) if need_x else None
+    dtype = x.dtype
+    dx = (torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=dtype, device=x.device)) if need_x else None
+    x, ld = _rows(x, x.shape[-1])
+    rows, D = x.shape
     if not rows:
         return dx, torch.zeros_like(weight) if need_w else None, torch.zeros_like(bias) if need_b else None, None
     g, ldg = _rows(dy if dy.dtype == dtype else dy.to(dtype), D)
+    w = _dense(weight)
     sw = accumulation_sink(ctx, 1, weight) if need_w and sinks else None
     sb = accumulation_sink(ctx, 1 if weight is None else 2, bias) if need_b and sinks else None
-    dw = sw if sw is not None else torch.empty(D, dtype=F32, device=dev) if need_w else None
-    db = sb if sb is not None else torch.empty(D, dtype=F32, device=dev) if need_b else None
+    dw = sw if sw is not None else x.new_empty(D, dtype=F32) if need_w else None
+    db = sb if sb is not None else x.new_empty(D, dtype=F32) if need_b else None
     bf16 = int(dtype == BF16)
     parts = lib().layer_norm_parts(bf16, rows, D)
-    part = torch.empty(parts * 2 * D, dtype=F32, device=dev) if need_w or need_b else None
+    part = x.new_empty(parts * 2 * D, dtype=F32) if need_w or need_b else None
     # (the engine runs a node on the device and stream of its forward pass)
-    lib().layer_norm_bwd(ptr(x), bf16, ld, ptr(g), ldg, ptr(w), ptr(stats), ptr(dx), ptr(part), parts, ptr(dw), ptr(db),
-                         int(sw is not None), int(sb is not None), rows, D, stream_handle())
+    lib().layer_norm_bwd(x.data_ptr(), bf16, ld, g.data_ptr(), ldg, ptr(w), stats.data_ptr(), ptr(dx), ptr(part), parts, ptr(dw),
+                         ptr(db), int(sw is not None), int(sb is not None), rows, D, stream_handle())
     return dx, None if sw is not None else dw, None if sb is not None else db, None
+
+
+_apply = fast_apply(_LayerNormFn)
 
 
 def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
@@ -120,5 +124,5 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     if len(shape) > 1:
         x2 = x.reshape(*x.shape[:-len(shape)], D)
         weight, bias = (t.reshape(D) if t is not None else None for t in (weight, bias))
-        return _LayerNormFn.apply(x2, weight, bias, float(eps)).reshape(x.shape)
-    return _LayerNormFn.apply(x, weight, bias, float(eps))
+        return _apply(x2, weight, bias, float(eps)).reshape(x.shape)
+    return _apply(x, weight, bias, float(eps))
