@@ -386,8 +386,10 @@ PYBIND11_MODULE(_C, m) {
 #undef XENT_ARGS
   m.attr("XENT_MAX_ROWS") = DV_XENT_MAX_ROWS;
   m.attr("XENT_MAX_CLASSES") = DV_XENT_MAX_CLASSES;
-  m.def("pack_rows", [](uptr src, int bf16, int64_t lds, int64_t rows, int cols, uptr dst, int64_t ldd, uptr st) {
-    if (dv_pack_rows(CP(src), bf16, lds, rows, cols, P(dst), ldd, ST(st))) throw std::runtime_error("pack_rows: unsupported shape");
+  m.def("pack_rows", [](uptr src0, int bf0, int64_t lds0, int64_t rows0, uptr dst0, uptr src1, int bf1, int64_t lds1,
+                        int64_t rows1, uptr dst1, int cols, int64_t ldd, uptr st) {
+    if (dv_pack_rows({CP(src0), bf0, cols, lds0, rows0, P(dst0), ldd}, {CP(src1), bf1, cols, lds1, rows1, P(dst1), ldd}, ST(st)))
+      throw std::runtime_error("pack_rows: unsupported shape");
     check_last("pack_rows");
   });
   m.attr("ADAMW_BLOCK") = DV_ADAMW_BLOCK;

@@ -281,8 +281,15 @@ int dv_linear_xent_fwd(const DvXent& a, void* ws, float* lse, float* loss_rows, 
 // wt: bf16 [width][ldwt] = w transposed, zeros behind V, or null
 int dv_linear_xent_bwd(const DvXent& a, void* ws, const float* lse, const void* wt, int64_t ldwt, void* dx, void* dw,
                        int dw_f32, int dw_add, float* db, int db_add, hipStream_t st);
-// bf16 [rows][ldd] = src [rows][cols] (row stride lds), zeros behind cols
-int dv_pack_rows(const void* src, int is_bf16, int64_t lds, int64_t rows, int cols, void* dst, int64_t ldd, hipStream_t st);
+// bf16 [rows][ldd] = src [rows][cols] (row stride lds), zeros behind cols; two matrices, no rows: none
+struct DvPack {
+  const void* src;
+  int bf16, cols;
+  int64_t lds, rows;
+  void* dst;
+  int64_t ldd;
+};
+int dv_pack_rows(const DvPack& m0, const DvPack& m1, hipStream_t st);
 
 // ---- layer norm (layer_norm.hip) ----
 // x / dy rows at strides ldx / ldg, y / dx dense; stats [rows][2] = mean, rstd; w / b / dw / db may be null.

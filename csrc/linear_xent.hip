@@ -234,19 +234,70 @@ __global__ __launch_bounds__(256) void total_kernel(const float2* __restrict__ b
 }
 
 // --------------------------------------------------------------------------------------- backward
+// dst[c][r] = src[r][c] for r < rows (by_label: only of counted rows), 0 up to ldd; 64 x 64 by 256 threads,
+// one or two matrices a launch. 16-byte loads and stores; a column of the LDS image is gathered by 2 bytes.
+struct Transpose {
+  const u16* src;
+  int64_t ld;
+  int rows, cols;
+  u16* dst;
+  int64_t ldd;
+  int by_label;
+  int blocks;  // (ldd / 64) x ceil(cols / 64)
+};
+constexpr int TRANSPOSE_LDS = 64 * 74 * 2;  // 37 banks a row: gathers of 8 rows apart do not meet
+DV_DEVICE void transpose_block(const DvXent& x, const Transpose& m0, const Transpose& m1, int id, int tid, char* smem) {
+  u16(*sh)[74] = reinterpret_cast<u16(*)[74]>(smem);
+  const bool any = id < m0.blocks + m1.blocks;
+  const Transpose& t = id < m0.blocks ? m0 : m1;
+  if (id >= m0.blocks) id -= m0.blocks;
+  const int across = any ? (int)(t.ldd / 64) : 1, r0 = id % across * 64, c0 = id / across * 64;
+  if (any) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {  // rows of the operand hold whole 64-column blocks (zeros from `width` on)
+      const int r = e * 32 + (tid >> 3), c = (tid & 7) * 8;
+      uint4 d{0, 0, 0, 0};
+      if (r0 + r < t.rows && (!t.by_label || counted(x.labels[r0 + r], x)))
+        d = *reinterpret_cast<const uint4*>(t.src + (int64_t)(r0 + r) * t.ld + c0 + c);
+      uint32_t* to = reinterpret_cast<uint32_t*>(&sh[r][c]);
+      to[0] = d.x; to[1] = d.y; to[2] = d.z; to[3] = d.w;
+    }
+  }
+  __syncthreads();
+  if (!any) return;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int c = e * 32 + (tid >> 3), r = (tid & 7) * 8;
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = (uint32_t)sh[r + 2 * k][c] | (uint32_t)sh[r + 2 * k + 1][c] << 16;
+    if (c0 + c < t.cols) *reinterpret_cast<uint4*>(t.dst + (int64_t)(c0 + c) * t.ldd + r0 + r) = uint4{w[0], w[1], w[2], w[3]};
+  }
+}
+__global__ __launch_bounds__(256) void transpose_kernel(DvXent x, Transpose m0, Transpose m1) {
+  __shared__ __attribute__((aligned(16))) char smem[TRANSPOSE_LDS];
+  transpose_block(x, m0, m1, blockIdx.x, threadIdx.x, smem);
+}
+
 // d of the piece [p0, p0 + pv) of the vocabulary: P [n][pvp], zero from pv on, and
 // Q = t . d [v][ldq], zero up to ldq; db partial sums [n block and wave][pv]
 template <class T, int BM, int BN, int WN>
 __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(DvXent a, const float2* __restrict__ lse, int p0,
                                                                               int pv, int pvp, u16* __restrict__ P,
                                                                               u16* __restrict__ Q, int64_t ldq,
-                                                                              float* __restrict__ pbias) {
+                                                                              float* __restrict__ pbias, int tiles,
+                                                                              Transpose m0, Transpose m1) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
+  if ((int)blockIdx.x >= tiles) {  // the blocks behind the tiles lay out what the next launch reads
+    const int sub = threadIdx.x >> 8;
+    transpose_block(a, m0, m1, (blockIdx.x - tiles) * (T::NTHREADS / 256) + sub, threadIdx.x & 255, smem + sub * TRANSPOSE_LDS);
+    return;
+  }
   constexpr int PITCH = 144;  // bytes: 64 bf16 + 16, conflict-free both ways
   constexpr int MG = T::TM < 2 ? 1 : 2, MW = 32 * MG, NW = 32 * T::TN;
   // tiles up to pvp and ldq: where a tile is half of 64 the last one may hold nothing but zeros of P or Q
   const int tm = (pvp + BM - 1) / BM, tn = (int)((ldq + BN - 1) / BN);
-  const TileAt at = tile_at(blockIdx.x, gridDim.x, tm, tn);
+  const TileAt at = tile_at(blockIdx.x, tiles, tm, tn);
   const int v0 = at.m * BM, n0 = at.n * BN;  // v: within the piece
   T t;
   t.run({a.w + (int64_t)(p0 + min(v0, pv - 1)) * a.ldw, a.ldw, max(pv - v0, 1)},
@@ -486,74 +537,42 @@ __global__ __launch_bounds__(256) void reduce_kernel(DvXent x, OutArgs g) {
   }
 }
 
-// dst[c][r] = src[r][c] for r < rows (by_label: only of counted rows), 0 up to ldd; 64 x 64 a block, one
-// or two matrices a launch. 16-byte loads and stores; a column of the LDS image is gathered by 2 bytes.
-struct Transpose {
-  const u16* src;
-  int64_t ld;
-  int rows, cols;
-  u16* dst;
-  int64_t ldd;
-  int by_label;
-  int blocks;  // (ldd / 64) x ceil(cols / 64)
-};
-__global__ __launch_bounds__(256) void transpose_kernel(DvXent x, Transpose m0, Transpose m1) {
-  __shared__ __attribute__((aligned(16))) u16 sh[64][74];  // 37 banks a row: gathers of 8 rows apart do not meet
-  int id = blockIdx.x;
-  const Transpose& t = id < m0.blocks ? m0 : m1;
-  if (id >= m0.blocks) id -= m0.blocks;
-  const int across = (int)(t.ldd / 64), r0 = id % across * 64, c0 = id / across * 64;
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {  // rows of the operand hold whole 64-column blocks (zeros from `width` on)
-    const int r = e * 32 + (threadIdx.x >> 3), c = (threadIdx.x & 7) * 8;
-    uint4 d{0, 0, 0, 0};
-    if (r0 + r < t.rows && (!t.by_label || counted(x.labels[r0 + r], x)))
-      d = *reinterpret_cast<const uint4*>(t.src + (int64_t)(r0 + r) * t.ld + c0 + c);
-    uint32_t* to = reinterpret_cast<uint32_t*>(&sh[r][c]);
-    to[0] = d.x; to[1] = d.y; to[2] = d.z; to[3] = d.w;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int c = e * 32 + (threadIdx.x >> 3), r = (threadIdx.x & 7) * 8;
-    uint32_t w[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = (uint32_t)sh[r + 2 * k][c] | (uint32_t)sh[r + 2 * k + 1][c] << 16;
-    if (c0 + c < t.cols) *reinterpret_cast<uint4*>(t.dst + (int64_t)(c0 + c) * t.ldd + r0 + r) = uint4{w[0], w[1], w[2], w[3]};
-  }
-}
-
-// dst [rows][ldd] bf16 = src [rows][cols] (bf16 or fp32), zero behind cols
+// dst [rows][ldd] bf16 = src [rows][cols] (bf16 or fp32), zero behind cols; one or two matrices a launch
 template <class S>
-__global__ __launch_bounds__(256) void pack_kernel(const S* __restrict__ src, int64_t lds_, int64_t rows, int cols,
-                                                   u16* __restrict__ dst, int64_t ldd) {
-  for (int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x; u < rows * (ldd / 8); u += (int64_t)gridDim.x * 256) {
-    const int64_t r = u / (ldd / 8);
-    const int c = (int)(u - r * (ldd / 8)) * 8;
-    const S* p = src + r * lds_ + c;
-    uint32_t w[4] = {};
-    if (c + 8 <= cols) {  // rows start at any element
-      if constexpr (sizeof(S) == 2) {
-        const u32x4_a2 q = *reinterpret_cast<const u32x4_a2*>(p);
+DV_DEVICE uint4 pack8(const S* p, int left) {
+  uint32_t w[4] = {};
+  if (left >= 8) {  // rows start at any element
+    if constexpr (sizeof(S) == 2) {
+      const u32x4_a2 q = *reinterpret_cast<const u32x4_a2*>(p);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = q[e];
-      } else {
-        const f32x4_a4 q0 = *reinterpret_cast<const f32x4_a4*>(p), q1 = *reinterpret_cast<const f32x4_a4*>(p + 4);
-        w[0] = pack2bf(q0[0], q0[1]); w[1] = pack2bf(q0[2], q0[3]);
-        w[2] = pack2bf(q1[0], q1[1]); w[3] = pack2bf(q1[2], q1[3]);
-      }
+      for (int e = 0; e < 4; ++e) w[e] = q[e];
     } else {
-      for (int e = 0; e < cols - c; ++e) {
-        uint32_t v;
-        if constexpr (sizeof(S) == 2) v = p[e];
-        else v = f2bf(p[e]);
-        const uint32_t at = v << (16 * (e & 1));
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (k == e >> 1) w[k] |= at;
-      }
+      const f32x4_a4 q0 = *reinterpret_cast<const f32x4_a4*>(p), q1 = *reinterpret_cast<const f32x4_a4*>(p + 4);
+      w[0] = pack2bf(q0[0], q0[1]); w[1] = pack2bf(q0[2], q0[3]);
+      w[2] = pack2bf(q1[0], q1[1]); w[3] = pack2bf(q1[2], q1[3]);
     }
-    *reinterpret_cast<uint4*>(dst + r * ldd + c) = uint4{w[0], w[1], w[2], w[3]};
+  } else {
+    for (int e = 0; e < left; ++e) {
+      uint32_t v;
+      if constexpr (sizeof(S) == 2) v = p[e];
+      else v = f2bf(p[e]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k == e >> 1) w[k] |= v << (16 * (e & 1));
+    }
+  }
+  return uint4{w[0], w[1], w[2], w[3]};
+}
+__global__ __launch_bounds__(256) void pack_kernel(DvPack m0, DvPack m1, int b0) {
+  const bool second = (int)blockIdx.x >= b0;
+  const DvPack& m = second ? m1 : m0;
+  const int64_t block = second ? blockIdx.x - b0 : blockIdx.x, grid = second ? gridDim.x - b0 : b0, per = m.ldd / 8;
+  for (int64_t u = block * 256 + threadIdx.x; u < m.rows * per; u += grid * 256) {
+    const int64_t r = u / per;
+    const int c = (int)(u - r * per) * 8;
+    const uint4 d = m.bf16 ? pack8(reinterpret_cast<const u16*>(m.src) + r * m.lds + c, m.cols - c)
+                           : pack8(reinterpret_cast<const float*>(m.src) + r * m.lds + c, m.cols - c);
+    *reinterpret_cast<uint4*>(reinterpret_cast<u16*>(m.dst) + r * m.ldd + c) = d;
   }
 }
 
@@ -741,14 +760,21 @@ int dv_linear_xent_bwd(const DvXent& a, void* ws, const float* lse, const void* 
     Transpose tx{}, tw{};
     if (need_w && p0 == 0) tx = transposed(a.x, a.ldx, a.N, xt, l.ldq, 1);
     if (need_x && !wt_all) tw = transposed(a.w + (int64_t)p0 * a.ldw, a.ldw, pv, wt, pvp, 0);
-    if (tx.blocks + tw.blocks) transpose_kernel<<<(unsigned)(tx.blocks + tw.blocks), 256, 0, st>>>(a, tx, tw);
+    // in the gradient's launch, but for the largest tiles: a block there takes a CU's LDS, whatever it does
+    // (8192 x 65536 x 2048: 50 us apart, 80 rounds of blocks within)
+    int beside = tx.blocks + tw.blocks;
+    if (beside && l.pg.form == 0) {
+      transpose_kernel<<<(unsigned)beside, 256, 0, st>>>(a, tx, tw);
+      beside = 0;
+    }
     with_tile(l.pg.form, [&](auto tile, auto bm, auto bn, auto, auto wn) {
       using T = decltype(tile);
       constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WN = decltype(wn)::value;
       static bool done[64];
       allow_lds(grad_kernel<T, BM, BN, WN>, T::LDS, done);
-      grad_kernel<T, BM, BN, WN><<<(unsigned)(cdiv(pvp, BM) * cdiv(l.ldq, BN)), T::NTHREADS, T::LDS, st>>>(a, reinterpret_cast<const float2*>(lse), p0, pv, pvp, P, Q,
-                                                                                                     l.ldq, pb);
+      const int tiles = cdiv(pvp, BM) * cdiv(l.ldq, BN), more = cdiv(beside, T::NTHREADS / 256);
+      grad_kernel<T, BM, BN, WN><<<(unsigned)(tiles + more), T::NTHREADS, T::LDS, st>>>(
+          a, reinterpret_cast<const float2*>(lse), p0, pv, pvp, P, Q, l.ldq, pb, tiles, tx, tw);
     });
     OutArgs gw{};
     if (need_x)
@@ -770,10 +796,16 @@ int dv_linear_xent_bwd(const DvXent& a, void* ws, const float* lse, const void* 
   return 0;
 }
 
-int dv_pack_rows(const void* src, int is_bf16, int64_t lds_, int64_t rows, int cols, void* dst, int64_t ldd, hipStream_t st) {
-  if (rows <= 0 || cols <= 0 || ldd % 8 || ldd < cols) return -1;
-  const unsigned grid = (unsigned)std::min<int64_t>((rows * (ldd / 8) + 255) / 256, 8192);
-  if (is_bf16) pack_kernel<u16><<<grid, 256, 0, st>>>((const u16*)src, lds_, rows, cols, (u16*)dst, ldd);
-  else pack_kernel<float><<<grid, 256, 0, st>>>((const float*)src, lds_, rows, cols, (u16*)dst, ldd);
+int dv_pack_rows(const DvPack& m0, const DvPack& m1, hipStream_t st) {
+  int grid[2];
+  const DvPack* all[2] = {&m0, &m1};
+  for (int i = 0; i < 2; ++i) {
+    const DvPack& m = *all[i];
+    grid[i] = 0;
+    if (!m.rows) continue;
+    if (m.rows < 0 || m.cols <= 0 || m.ldd % 8 || m.ldd < m.cols || m.lds < m.cols) return -1;
+    grid[i] = (int)std::min<int64_t>((m.rows * (m.ldd / 8) + 255) / 256, 8192);
+  }
+  if (grid[0] + grid[1]) pack_kernel<<<(unsigned)(grid[0] + grid[1]), 256, 0, st>>>(m0, m1, grid[0]);
   return 0;
 }

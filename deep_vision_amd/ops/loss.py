@@ -72,16 +72,27 @@ def _linear_xent_plain(x, weight, labels, bias, smoothing, ignore_index, reducti
     return rows.sum() / max(rows.numel(), 1) if reduction == "mean" else rows.sum()
 
 
-def _bf16_rows(t, D, Dp):
-    """``t`` [rows][D] as a bf16 operand of the products: rows of Dp columns (zeros behind D) on 16 bytes.
-    The tensor itself where it is one already."""
-    if t.dtype == BF16 and D == Dp and t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0 and \
-            D <= t.stride(0) <= 1 << 22:
-        return t
-    if t.stride(1) != 1 or t.stride(0) < D:
-        t = t.contiguous()
-    out = torch.empty((t.shape[0], Dp), dtype=BF16, device=t.device)
-    lib().pack_rows(ptr(t), int(t.dtype == BF16), t.stride(0), t.shape[0], D, ptr(out), Dp, stream_handle())
+def _is_operand(t, D, Dp):
+    return (t.dtype == BF16 and D == Dp and t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
+            and D <= t.stride(0) <= 1 << 22)
+
+
+def _operands(x, weight, D, Dp):
+    """x and weight (None: not wanted) as bf16 operands of the products: rows of Dp columns (zeros behind D) on
+    16 bytes. A tensor that is one already itself, the others packed in one launch."""
+    out, args = [], []
+    for t in (x, weight):
+        if t is None or _is_operand(t, D, Dp):
+            out.append(t)
+            args += (0, 0, 0, 0, 0)
+            continue
+        if t.stride(1) != 1 or t.stride(0) < D:
+            t = t.contiguous()
+        k = t.new_empty((t.shape[0], Dp), dtype=BF16)
+        out.append(k)
+        args += (ptr(t), int(t.dtype == BF16), max(t.stride(0), D), t.shape[0], ptr(k))
+    if any(args):
+        lib().pack_rows(*args, D, Dp, stream_handle())
     return out
 
 
@@ -115,9 +126,10 @@ def _linear_xent_forward(x, weight, bias, labels, smoothing, ignore_index, reduc
     N, D = x.shape
     V, dev = weight.shape[0], x.device
     Dp = (D + 63) // 64 * 64
-    xk = _bf16_rows(x, D, Dp)
     cached = _cached_weight(weight)
-    wk = _operand(weight, Dp) if cached else _bf16_rows(weight, D, Dp)
+    xk, wk = _operands(x, None if cached else weight, D, Dp)
+    if cached:
+        wk = _operand(weight, Dp)
     b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     args = _linear_xent_args(xk, wk, b, labels, V, Dp, D, ignore_index, smoothing, reduction)
     ws = torch.empty(lib().linear_xent_fwd_bytes(*args), dtype=torch.uint8, device=dev)
