@@ -372,6 +372,7 @@ PYBIND11_MODULE(_C, m) {
       throw std::runtime_error("linear_xent_fwd: unsupported shape");
     check_last("linear_xent_fwd");
   });
+  m.def("linear_xent_reads_wt", [](XENT_ARGS) { return dv_linear_xent_reads_wt(XENT(0, 0)); });
   m.def("linear_xent_bwd_bytes", [](XENT_ARGS, int need_x, int need_w, int need_b, int have_wt) {
     return dv_linear_xent_bwd_bytes(XENT(0, 0), need_x, need_w, need_b, have_wt);
   });

@@ -10,12 +10,14 @@
 //
 //  * forward: one product whose epilogue leaves (max, sum of exponentials) of every row over the
 //    columns of one wave; a second launch joins them.
-//  * backward, for each piece of the vocabulary: the product again, its epilogue writes d in bf16 both
-//    ways round ([n][v] and [v][n]), because each of the two products that follow wants its own sum
-//    index contiguous; then dx += d w and dw = d' x. x' and the piece of w' are laid out once a call.
+//  * backward, for each piece of the vocabulary: the product again, its epilogue writes d in bf16; then
+//    dx += d w and dw = d' x, whose sums run over the classes and over the rows. The largest tiles read w
+//    and d k by k, as they lie (gemm_tile.h); the smaller ones lose more to that than they save, so d is
+//    written both ways round for them and w' laid out once a call. x' is laid out for both. 8192 x 65536
+//    x 2048: 7.41 -> 7.02 ms with w and d as they lie.
 //  * d is rounded to bf16 before it is scaled (and divided by 1 - e): a label's entry p - 1 then rounds the
-//    same whatever the batch size, and the scale is applied to the fp32 sums. Only with an upstream gradient for each row
-//    does d' carry it (the sum over n cannot).
+//    same whatever the batch size, and the scale is applied to the fp32 sums. Only an upstream gradient for
+//    each row goes into d, since the sum over n cannot apply it.
 //  * a row whose label is ignored (or lies outside [0, V)) takes no part: its d is zero and so is its
 //    row of x', whatever x holds there.
 //  * sums that split an axis go through fp32 slabs added in a fixed order: no atomics, the same bits
@@ -24,12 +26,21 @@
 #include "kernels.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 using Big = GemmTile<256, 256, 2, 4>;
 using Mid = GemmTile<128, 128, 2, 2>;
 using Small = GemmTile<64, 64, 2, 2>;
 using Thin = ThinTile;
+// the tiles of dx (w read [v][k]) and of dw (d read [n][v])
+template <class T>
+struct OutTiles { using X = T; using W = T; };
+template <>
+struct OutTiles<Big> {
+  using X = GemmTile<256, 256, 2, 4, true, false>;
+  using W = GemmTile<256, 256, 2, 4, false, true>;
+};
 
 constexpr int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 constexpr int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
@@ -279,8 +290,8 @@ __global__ __launch_bounds__(256) void transpose_kernel(DvXent x, Transpose m0, 
   transpose_block(x, m0, m1, blockIdx.x, threadIdx.x, smem);
 }
 
-// d of the piece [p0, p0 + pv) of the vocabulary: P [n][pvp], zero from pv on, and
-// Q = t . d [v][ldq], zero up to ldq; db partial sums [n block and wave][pv]
+// d (times t, where each row has a gradient of its own) of the piece [p0, p0 + pv) of the vocabulary:
+// P [n][pvp], zero from pv and from N on, and Q [v][ldq], or null; db partial sums [n block and wave][pv]
 template <class T, int BM, int BN, int WN>
 __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(DvXent a, const float2* __restrict__ lse, int p0,
                                                                               int pv, int pvp, u16* __restrict__ P,
@@ -306,14 +317,12 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(Dv
   add_bias<T, BM>(t, a, p0 + v0);
   const float inv = 1.f / unit(a), off = a.smooth / a.V * inv, hot = a.smooth < 1.f ? 1.f : 0.f;
   const int vw0 = p0 + v0 + t.wm * T::TM * 32;
-  float ts[T::TN];
 #pragma unroll
   for (int j = 0; j < T::TN; ++j) {
     const int n = n0 + t.col(j);
     const int64_t label = n < a.N ? a.labels[n] : -1;
     const bool use = n < a.N && counted(label, a);
     const float2 z = use ? lse[n] : float2{0.f, 0.f};
-    ts[j] = use ? (a.reduction == DV_XENT_NONE ? a.go[n] : 1.f) : 0.f;
 #pragma unroll
     for (int i = 0; i < T::TM; ++i)
 #pragma unroll
@@ -325,6 +334,13 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(Dv
       for (int i = 0; i < T::TM; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) t.acc[i][j][r] -= rel == i * 32 + (r & 3) + 8 * (r >> 2) ? hot : 0.f;
+    }
+    if (a.reduction == DV_XENT_NONE) {
+      const float row = use ? a.go[n] : 0.f;
+#pragma unroll
+      for (int i = 0; i < T::TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) t.acc[i][j][r] *= row;
     }
     if (__any(!use)) {  // whatever x holds in rows that do not count
 #pragma unroll
@@ -346,7 +362,7 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(Dv
       for (int r = 0; r < 16; ++r) {
         float s = 0.f;
 #pragma unroll
-        for (int j = 0; j < T::TN; ++j) s += t.acc[i][j][r] * ts[j];
+        for (int j = 0; j < T::TN; ++j) s += t.acc[i][j][r];
         s = row16_sum(s);
         s += __shfl_xor(s, 16, 64);
         const int v = v0 + t.row(i, r);
@@ -377,7 +393,7 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(Dv
     for (int e = 0; e < NW * MW / 512; ++e) {
       const int w = e * 64 + t.lane, n = w / (MW / 8), c = w % (MW / 8) * 8;
       const uint4 d = *reinterpret_cast<const uint4*>(mine + n * PITCH + c * 2);
-      if (nw + n < a.N && vw + c < pvp) *reinterpret_cast<uint4*>(P + (int64_t)(nw + n) * pvp + vw + c) = d;
+      if (nw + n < ldq && vw + c < pvp) *reinterpret_cast<uint4*>(P + (int64_t)(nw + n) * pvp + vw + c) = d;
     }
     wave_sync();
     if (Q) {
@@ -387,12 +403,7 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(Dv
         for (int i = 0; i < MG; ++i)
 #pragma unroll
           for (int k = 0; k < 8; ++k) {  // columns v, v + 1 of two neighbouring rows n become rows of Q
-            uint32_t w = u[i][j][k];
-            if (a.reduction == DV_XENT_NONE) {
-              const f32x16& c = t.acc[h * MG + i][j];
-              w = pack2bf(c[2 * k] * ts[j], c[2 * k + 1] * ts[j]);
-            }
-            const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0xB1, 0xF, 0xF, false);  // lane ^ 1
+            const uint32_t w = u[i][j][k], o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0xB1, 0xF, 0xF, false);  // lane ^ 1
             const int v = i * 32 + (k & 1) * 2 + 8 * (k >> 1) + 4 * (t.lane >> 5) + (t.lane & 1);
             *reinterpret_cast<uint32_t*>(mine + v * PITCH + (j * 32 + (t.lane & 30)) * 2) = __builtin_amdgcn_perm(w, o, swap);
           }
@@ -417,16 +428,15 @@ struct OutArgs {
   int slab_add;
   void* out;         // [N][M], bf16 or fp32
   int out_f32, out_add;
-  int by_row;        // the scale is that of row n (0 where its label does not count)
+  int by_row;        // 0 in rows n whose label does not count
+  int deep;          // valid k of `a`, where the tile reads it [k][m]
 };
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
 typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 
 DV_DEVICE float out_scale(const DvXent& x, bool by_row, int64_t n, float common) {
-  if (!by_row) return common;
-  if (!counted(x.labels[n], x)) return 0.f;
-  return x.reduction == DV_XENT_NONE ? x.go[n] * common : common;
+  return !by_row || counted(x.labels[n], x) ? common : 0.f;
 }
 DV_DEVICE void put4(void* out, int f32, int add, int64_t o, int left, f32x4 v) {
   if (f32) {
@@ -465,26 +475,20 @@ DV_DEVICE void fold_bias(const DvXent& x, const BiasArgs& b, int block, float* s
   }
 }
 
-// The products behind a piece's d, and the fold of its bias gradient, in one launch: blocks
-// [0, b0) compute g0, [b0, b0 + b1) g1, the rest the bias.
+// tile `id` of g
 template <class T, int BM, int BN>
-__global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void out_kernel(DvXent x, OutArgs g0, OutArgs g1, BiasArgs bias,
-                                                                             int b0, int b1) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+DV_DEVICE void out_tile(const DvXent& x, const OutArgs& g, int id, char* smem) {
   constexpr int PITCH = 144, NW = 32 * T::TN;
-  int id = blockIdx.x;
-  if (id >= b0 + b1) return fold_bias(x, bias, id - b0 - b1, reinterpret_cast<float*>(smem));
-  const bool second = id >= b0;
-  const OutArgs& g = second ? g1 : g0;
-  if (second) id -= b0;
   const int tm = (g.M + BM - 1) / BM, tn = (g.N + BN - 1) / BN;
   const int tiles = tm * tn, split = id / tiles;
   const TileAt at = tile_at(id - split * tiles, tiles, tm, tn);
   const int m0 = at.m * BM, n0 = at.n * BN;
   const int k0 = (int)((int64_t)g.ktiles * split / g.splits), k1 = (int)((int64_t)g.ktiles * (split + 1) / g.splits);
+  GemmOperand a{g.a + (int64_t)m0 * g.lda + k0 * 64, g.lda, g.M - m0}, b{g.b + (int64_t)n0 * g.ldb + k0 * 64, g.ldb, g.N - n0};
+  if constexpr (T::TURNED_A) a = {g.a + (int64_t)k0 * 64 * g.lda + m0, g.lda, g.M - m0, g.deep - k0 * 64};
+  if constexpr (T::TURNED_B) b = {g.b + (int64_t)k0 * 64 * g.ldb + n0, g.ldb, g.N - n0, (g.ktiles - k0) * 64};
   T t;
-  t.run({g.a + (int64_t)m0 * g.lda + k0 * 64, g.lda, g.M - m0}, {g.b + (int64_t)n0 * g.ldb + k0 * 64, g.ldb, g.N - n0},
-        k1 - k0, smem);
+  t.run(a, b, k1 - k0, smem);
   if (!t.active()) return;
   const float common = g.slab ? 1.f : common_scale(x);
   char* mine = smem + t.wave * NW * PITCH;
@@ -515,6 +519,21 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void out_kernel(DvX
     }
     wave_sync();
   }
+}
+
+// The products behind a piece's d, and the fold of its bias gradient, in one launch: blocks [0, b0) compute
+// dx, [b0, b0 + b1) dw, the rest the bias.
+template <class T, int BM, int BN>
+__global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void out_kernel(DvXent x, OutArgs gx, OutArgs gw, BiasArgs bias,
+                                                                             int b0, int b1) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  using X = typename OutTiles<T>::X;
+  using W = typename OutTiles<T>::W;
+  const int id = blockIdx.x;
+  if (id >= b0 + b1) return fold_bias(x, bias, id - b0 - b1, reinterpret_cast<float*>(smem));
+  if constexpr (std::is_same_v<X, W>) out_tile<T, BM, BN>(x, id < b0 ? gx : gw, id < b0 ? id : id - b0, smem);
+  else if (id < b0) out_tile<X, BM, BN>(x, gx, id, smem);
+  else out_tile<W, BM, BN>(x, gw, id - b0, smem);
 }
 
 // out[n][m] = scale * sum over splits of the slab
@@ -652,36 +671,48 @@ FwdLayout fwd_layout(const DvXent& a) {
 struct BwdLayout {
   int piece;           // columns of the vocabulary at a time
   Plan pg, px, pw;     // the logits again, dx, dw
+  bool direct;         // the products read w [v][k] and d [n][v]: no w', no second layout of d
   int64_t ldq;
   int bias_parts;
   bool dx_slab;
   int64_t P, Q, xt, wt, sx, sw, pb, bytes;
 };
-constexpr int64_t PIECE_BYTES = 1LL << 30;  // both layouts of a piece's d
+constexpr int64_t PIECE_BYTES = 1LL << 30;  // a piece's d, in the layouts that are written
 BwdLayout bwd_layout(const DvXent& a, bool need_x, bool need_w, bool need_b, bool have_wt) {
   BwdLayout l;
   l.ldq = up(a.N, 64);
-  const int64_t most = std::max<int64_t>(PIECE_BYTES / (4 * l.ldq) / 256 * 256, 256);
-  const int pieces = cdiv(a.V, most);
-  l.piece = (int)std::min<int64_t>(up(cdiv(a.V, pieces), 256), a.V);
-  l.pg = plan(l.piece, a.N, a.D / 64, GRAD);
+  int pieces = 1;
+  auto cut = [&](int layouts) {
+    const int64_t most = std::max<int64_t>(PIECE_BYTES / (2 * layouts * l.ldq) / 256 * 256, 256);
+    pieces = cdiv(a.V, most);
+    l.piece = (int)std::min<int64_t>(up(cdiv(a.V, pieces), 256), a.V);
+  };
+  auto dx_plan = [&](int f) { return plan_form(f, a.width, a.N, cdiv(l.piece, 64), true, PLAIN); };
+  auto dw_plan = [&](int f) { return plan_form(f, a.width, l.piece, cdiv(a.N, 64), true, PLAIN); };
   // dx and dw run in one launch and share a tile form, whichever of them is wanted: a gradient's bits do
   // not depend on which others are asked for
+  cut(2);
   double least = 1e30;
   for (int f = 0; f < FORMS; ++f) {
-    const Plan x = plan_form(f, a.width, a.N, cdiv(l.piece, 64), true, PLAIN),
-               w = plan_form(f, a.width, l.piece, cdiv(a.N, 64), true, PLAIN);
+    const Plan x = dx_plan(f), w = dw_plan(f);
     if (x.us + w.us < least) { least = x.us + w.us; l.px = x; l.pw = w; }
   }
+  l.direct = l.px.form == 0;
+  if (l.direct) {
+    cut(1);
+    l.px = dx_plan(0);
+    l.pw = dw_plan(0);
+  }
+  l.pg = plan(l.piece, a.N, a.D / 64, GRAD);
   l.bias_parts = cdiv(l.ldq, FORM_N[l.pg.form]) * FORM_WN[l.pg.form];
   l.dx_slab = l.px.splits > 1 || pieces > 1;
   const int64_t pvp = up(l.piece, 64);
   int64_t at = 0;
   auto take = [&](int64_t b) { const int64_t o = at; at += up(b, 256); return o; };
-  l.P = take((int64_t)a.N * pvp * 2);
-  l.Q = take(need_w ? (int64_t)l.piece * l.ldq * 2 : 0);
+  l.P = take(l.ldq * pvp * 2);
+  l.Q = take(need_w && !l.direct ? (int64_t)l.piece * l.ldq * 2 : 0);
   l.xt = take(need_w ? (int64_t)a.width * l.ldq * 2 : 0);
-  l.wt = take(need_x && !have_wt ? (int64_t)a.width * pvp * 2 : 0);
+  l.wt = take(need_x && !have_wt && !l.direct ? (int64_t)a.width * pvp * 2 : 0);
   l.sx = take(need_x && l.dx_slab ? (int64_t)l.px.splits * a.N * a.width * 4 : 0);
   l.sw = take(need_w && l.pw.splits > 1 ? (int64_t)l.pw.splits * l.piece * a.width * 4 : 0);
   l.pb = take(need_b ? (int64_t)l.bias_parts * l.piece * 4 : 0);
@@ -719,6 +750,8 @@ int64_t dv_linear_xent_bwd_bytes(const DvXent& a, int need_x, int need_w, int ne
   return bwd_layout(a, need_x, need_w, need_b, have_wt).bytes;
 }
 
+int dv_linear_xent_reads_wt(const DvXent& a) { return !bwd_layout(a, true, true, true, true).direct; }
+
 int dv_linear_xent_fwd(const DvXent& a, void* ws, float* lse, float* loss_rows, float* total, float* out, hipStream_t st) {
   if (!sane(a)) return -1;
   const FwdLayout l = fwd_layout(a);
@@ -748,7 +781,7 @@ int dv_linear_xent_bwd(const DvXent& a, void* ws, const float* lse, const void* 
   const bool need_w = dw != nullptr, need_x = dx != nullptr;
   const BwdLayout l = bwd_layout(a, need_x, need_w, db != nullptr, wt_all != nullptr);
   char* w = reinterpret_cast<char*>(ws);
-  u16 *P = reinterpret_cast<u16*>(w + l.P), *Q = need_w ? reinterpret_cast<u16*>(w + l.Q) : nullptr;
+  u16 *P = reinterpret_cast<u16*>(w + l.P), *Q = need_w && !l.direct ? reinterpret_cast<u16*>(w + l.Q) : nullptr;
   u16 *xt = reinterpret_cast<u16*>(w + l.xt), *wt = reinterpret_cast<u16*>(w + l.wt);
   float* pb = db ? reinterpret_cast<float*>(w + l.pb) : nullptr;
   auto transposed = [&](const u16* src, int64_t ld, int rows, u16* dst, int64_t ldd, int by_label) {
@@ -759,7 +792,7 @@ int dv_linear_xent_bwd(const DvXent& a, void* ws, const float* lse, const void* 
     const int pv = std::min(l.piece, a.V - p0), pvp = (int)up(pv, 64);
     Transpose tx{}, tw{};
     if (need_w && p0 == 0) tx = transposed(a.x, a.ldx, a.N, xt, l.ldq, 1);
-    if (need_x && !wt_all) tw = transposed(a.w + (int64_t)p0 * a.ldw, a.ldw, pv, wt, pvp, 0);
+    if (need_x && !wt_all && !l.direct) tw = transposed(a.w + (int64_t)p0 * a.ldw, a.ldw, pv, wt, pvp, 0);
     // in the gradient's launch, but for the largest tiles: a block there takes a CU's LDS, whatever it does
     // (8192 x 65536 x 2048: 50 us apart, 80 rounds of blocks within)
     int beside = tx.blocks + tw.blocks;
@@ -777,13 +810,15 @@ int dv_linear_xent_bwd(const DvXent& a, void* ws, const float* lse, const void* 
           a, reinterpret_cast<const float2*>(lse), p0, pv, pvp, P, Q, l.ldq, pb, tiles, tx, tw);
     });
     OutArgs gw{};
-    if (need_x)
-      gx = OutArgs{wt_all ? reinterpret_cast<const u16*>(wt_all) + p0 : wt, P, wt_all ? ldwt : pvp, pvp, a.width, a.N, pvp / 64,
-                   std::min(l.px.splits, pvp / 64), l.dx_slab ? reinterpret_cast<float*>(w + l.sx) : nullptr, p0 > 0, dx, 0, 0, 1};
+    if (need_x) {
+      const u16* rows = l.direct ? a.w + (int64_t)p0 * a.ldw : wt_all ? reinterpret_cast<const u16*>(wt_all) + p0 : wt;
+      gx = OutArgs{rows, P, l.direct ? a.ldw : wt_all ? ldwt : pvp, pvp, a.width, a.N, pvp / 64, std::min(l.px.splits, pvp / 64),
+                   l.dx_slab ? reinterpret_cast<float*>(w + l.sx) : nullptr, p0 > 0, dx, 0, 0, 1, pv};
+    }
     if (need_w) {
       char* to = reinterpret_cast<char*>(dw) + (int64_t)p0 * a.width * (dw_f32 ? 4 : 2);
-      gw = OutArgs{xt, Q, l.ldq, l.ldq, a.width, pv, (int)(l.ldq / 64), l.pw.splits,
-                   l.pw.splits > 1 ? reinterpret_cast<float*>(w + l.sw) : nullptr, 0, to, dw_f32, dw_add, 0};
+      gw = OutArgs{xt, l.direct ? P : Q, l.ldq, l.direct ? pvp : l.ldq, a.width, pv, (int)(l.ldq / 64), l.pw.splits,
+                   l.pw.splits > 1 ? reinterpret_cast<float*>(w + l.sw) : nullptr, 0, to, dw_f32, dw_add, 0, 0};
     }
     const BiasArgs gb{pb, l.bias_parts, pv, db ? db + p0 : nullptr, db_add};
     launch_out(a, l.px.form, gx, gw, gb, st);

@@ -174,11 +174,12 @@ def _linear_xent_backward(ctx, go, sinks):
         go = go.to(F32).contiguous()
     # (the engine runs a node on the device and stream of its forward pass)
     wt, Vp = None, (V + 63) // 64 * 64
-    if wk is None:  # the parameter's cached operands, as they are now
+    cached = wk is None
+    if cached:  # the parameter's operands, as they are now
         wk = _operand(weight, Dp)
-        if need_x and Vp <= 1 << 22:
-            wt = _transposed_operand(weight, Vp)
     args = _linear_xent_args(xk, wk, b, labels, V, Dp, D, ignore_index, smoothing, reduction)
+    if cached and need_x and Vp <= 1 << 22 and lib().linear_xent_reads_wt(*args):
+        wt = _transposed_operand(weight, Vp)
     ws = x.new_empty(lib().linear_xent_bwd_bytes(*args, int(need_x), int(need_w), int(need_b), int(wt is not None)),
                      dtype=torch.uint8)
     at = stats.data_ptr()

@@ -172,6 +172,36 @@ def test_several_pieces_of_the_vocabulary():
     run_and_check(*make(4096, 64, 70000, bias=True, ignored=0.1))
 
 
+# enough work that the products read the weight and the logits' gradient k by k
+@gpu
+@pytest.mark.parametrize("N,D,V,reduction", [(999, 2045, 8191, "none"), (2001, 1021, 16381, "mean"), (8101, 1500, 1999, "sum"),
+                                             (2001, 2048, 8190, "none")])
+def test_large_shapes_with_odd_ends(N, D, V, reduction):
+    x, w, b, y = make(N, D, V, bias=True, ignored=0.15)
+    go = torch.randn(N, device=DEV) if reduction == "none" else None
+    run_and_check(x, w, b, y, 0.1, reduction=reduction, go=go)
+    clean = F.linear_cross_entropy(x.requires_grad_(), w.requires_grad_(), y, reduction=reduction)
+    want = torch.autograd.grad(clean, (x, w), go)
+    x = x.detach().clone()
+    x[(y == -100).nonzero()[::2, 0]] = float("nan")  # whatever the rows hold that do not count
+    # a weight in the middle of a buffer of NaN: nothing beside it takes part
+    Dp = (D + 7) // 8 * 8
+    hold = torch.full((V + 70, Dp + 64), float("nan"), dtype=BF16, device=DEV)
+    inner = hold[3:V + 3, 8:8 + D]
+    inner.copy_(w.detach())
+    inner.requires_grad_()
+    got = torch.autograd.grad(F.linear_cross_entropy(x.requires_grad_(), inner, y, reduction=reduction), (x, inner), go)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    p = torch.nn.Parameter(w.detach().float())
+    got = torch.autograd.grad(F.linear_cross_entropy(x.nan_to_num(), p, y, reduction=reduction), p, go)[0]
+    assert torch.equal(got.to(BF16), want[1])
+
+
+@gpu
+def test_several_large_pieces_with_odd_ends():
+    run_and_check(*make(12001, 1021, 45007, bias=True, ignored=0.1))
+
+
 @gpu
 def test_wide_logits_and_classes_that_are_ruled_out():
     x, w, b, y = make(70, 64, 900, logit=40.0)
