@@ -372,14 +372,12 @@ PYBIND11_MODULE(_C, m) {
       throw std::runtime_error("linear_xent_fwd: unsupported shape");
     check_last("linear_xent_fwd");
   });
-  m.def("linear_xent_reads_wt", [](XENT_ARGS) { return dv_linear_xent_reads_wt(XENT(0, 0)); });
-  m.def("linear_xent_bwd_bytes", [](XENT_ARGS, int need_x, int need_w, int need_b, int have_wt) {
-    return dv_linear_xent_bwd_bytes(XENT(0, 0), need_x, need_w, need_b, have_wt);
+  m.def("linear_xent_bwd_bytes", [](XENT_ARGS, int need_x, int need_w, int need_b) {
+    return dv_linear_xent_bwd_bytes(XENT(0, 0), need_x, need_w, need_b);
   });
-  m.def("linear_xent_bwd", [](XENT_ARGS, uptr go, uptr total, uptr ws, uptr lse, uptr wt, int64_t ldwt, uptr dx, uptr dw,
-                              int dw_f32, int dw_add, uptr db, int db_add, uptr st) {
-    if (dv_linear_xent_bwd(XENT(go, total), P(ws), CFP(lse), CP(wt), ldwt, P(dx), P(dw), dw_f32, dw_add, FP(db), db_add,
-                           ST(st)))
+  m.def("linear_xent_bwd", [](XENT_ARGS, uptr go, uptr total, uptr ws, uptr lse, uptr dx, uptr dw, int dw_f32,
+                              int dw_add, uptr db, int db_add, uptr st) {
+    if (dv_linear_xent_bwd(XENT(go, total), P(ws), CFP(lse), P(dx), P(dw), dw_f32, dw_add, FP(db), db_add, ST(st)))
       throw std::runtime_error("linear_xent_bwd: unsupported shape");
     check_last("linear_xent_bwd");
   });

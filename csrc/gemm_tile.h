@@ -16,8 +16,8 @@
 //
 // An operand may also lie the other way round, [k][row] (KA, KB): its image is then [k][row] too, and
 // ds_read_b64_tr_b16 gives each lane four k of its row. 16 lanes read 4 rows of k by 32 bytes; the 64-byte
-// units of an LDS row are exclusive-or swizzled by k & 3, so that the lanes of a half wave touch all 64
-// banks once. 8192^3: 1345 TFLOP/s with KA, 1370 with KB; tiles of 128 lose 6 % to it (582 -> 545).
+// units of an LDS row are exclusive-or swizzled by k, so that the lanes of a half wave touch all 64 banks
+// once. 8192^3: 1345 TFLOP/s with KA, 1370 with KB.
 #pragma once
 #include "common.h"
 
@@ -32,13 +32,11 @@ struct GemmOperand {
 
 template <int BM, int BN, int WM, int WN, bool KA = false, bool KB = false>
 struct GemmTile {
-  static constexpr bool TURNED_A = KA, TURNED_B = KB;
   static constexpr int NW = WM * WN, NTHREADS = 64 * NW;
   static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
   static constexpr int BK = 64, STAGE = (BM + BN) * BK * 2, LDS = 2 * STAGE;
   static constexpr int IA = BM / 8 / NW, IB = BN / 8 / NW;  // 1-KB pieces (8 rows) a wave loads
   static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && BM % (32 * WM) == 0 && BN % (32 * WN) == 0, "tile");
-  static_assert((!KA || BM % 128 == 0) && (!KB || BN % 128 == 0), "the swizzle takes four units of 32 rows");
 
   f32x16 acc[TM][TN];
   int lane, wave, wm, wn;
@@ -63,6 +61,9 @@ struct GemmTile {
     asm volatile("" ::: "memory");
   }
 
+  // what the 64-byte units of row k are swizzled by: rows of 256 bytes or more, of 128 bytes
+  template <int B>
+  static DV_DEVICE int unit_swizzle(int k) { return B >= 128 ? k & 3 : (k >> 1) & 1; }
   // byte offsets, from a K-tile's start, of the 16 bytes this lane loads for each of its pieces
   template <bool K, int B, int I>
   DV_DEVICE void offsets(const GemmOperand& o, int deep, uint32_t (&off)[I]) const {
@@ -70,7 +71,7 @@ struct GemmTile {
     for (int i = 0; i < I; ++i) {
       if constexpr (K) {
         const int at = (wave * I + i) * 64 + lane, k = at / (B / 8), c = at % (B / 8);
-        const int row = (c ^ ((k & 3) << 2)) * 8;
+        const int row = (c ^ (unit_swizzle<B>(k) << 2)) * 8;
         off[i] = (uint32_t)(min(k, deep - 1) * o.ld * 2) + (uint32_t)min(row, (o.rows - 1) & ~7) * 2;
       } else {
         const int r = (wave * I + i) * 8 + (lane >> 3);
@@ -85,7 +86,7 @@ struct GemmTile {
     const int k = (lane & 15) >> 2;
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-      if constexpr (K) at[i] = ((lane >> 5) * 8 + k) * B * 2 + (((w * T + i) ^ k) << 6) + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+      if constexpr (K) at[i] = ((lane >> 5) * 8 + k) * B * 2 + (((w * T + i) ^ unit_swizzle<B>(k)) << 6) + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
       else at[i] = (w * T * 32 + (lane & 31)) * 128;
     }
   }
@@ -201,7 +202,6 @@ struct GemmTile {
 // the waves meet once at the end. The first wave holds the result. Logits and their statistics of 8 rows by
 // 1000 columns, sum of 2048: 7.6 us, of 256 rows 9.8 us; in 64 x 64 tiles, a chain of 32 K-tiles, 11.7 and 18.6.
 struct ThinTile {
-  static constexpr bool TURNED_A = false, TURNED_B = false;
   static constexpr int NW = 8, NTHREADS = 512, TM = 1, TN = 1, BK = 64, IMAGE = 64 * 128, LDS = NW * IMAGE;
 
   f32x16 acc[1][1];

@@ -274,14 +274,12 @@ struct DvXent {
   const float* total;      // backward, mean: [1] is the number of rows that count
 };
 int64_t dv_linear_xent_fwd_bytes(const DvXent& a);
-int dv_linear_xent_reads_wt(const DvXent& a);
-int64_t dv_linear_xent_bwd_bytes(const DvXent& a, int need_x, int need_w, int need_b, int have_wt);
+int64_t dv_linear_xent_bwd_bytes(const DvXent& a, int need_x, int need_w, int need_b);
 // lse [N][2] (backward's; largest logit, log2 of the sum above it) and loss_rows [N] may be null; out (the reduced loss) and total [2] go together, null for DV_XENT_NONE
 int dv_linear_xent_fwd(const DvXent& a, void* ws, float* lse, float* loss_rows, float* total, float* out, hipStream_t st);
 // dx [N][width] bf16, dw [V][width] bf16 or fp32 (added to where dw_add), db [V]; each may be null.
-// wt: bf16 [width][ldwt] = w transposed, zeros behind V, or null; of no use where not reads_wt
-int dv_linear_xent_bwd(const DvXent& a, void* ws, const float* lse, const void* wt, int64_t ldwt, void* dx, void* dw,
-                       int dw_f32, int dw_add, float* db, int db_add, hipStream_t st);
+int dv_linear_xent_bwd(const DvXent& a, void* ws, const float* lse, void* dx, void* dw, int dw_f32, int dw_add, float* db,
+                       int db_add, hipStream_t st);
 // bf16 [rows][ldd] = src [rows][cols] (row stride lds), zeros behind cols; two matrices, no rows: none
 struct DvPack {
   const void* src;

@@ -11,10 +11,10 @@
 //  * forward: one product whose epilogue leaves (max, sum of exponentials) of every row over the
 //    columns of one wave; a second launch joins them.
 //  * backward, for each piece of the vocabulary: the product again, its epilogue writes d in bf16; then
-//    dx += d w and dw = d' x, whose sums run over the classes and over the rows. The largest tiles read w
-//    and d k by k, as they lie (gemm_tile.h); the smaller ones lose more to that than they save, so d is
-//    written both ways round for them and w' laid out once a call. x' is laid out for both. 8192 x 65536
-//    x 2048: 7.41 -> 7.02 ms with w and d as they lie.
+//    dx += d w and dw = d' x, whose sums run over the classes and over the rows. Both operands whose sum index
+//    is not the contiguous one, w and d, are read k by k as they lie (gemm_tile.h); d written both ways round and
+//    w' laid out cost 8192 x 65536 x 2048 7.41 ms against 7.02, 2048 x 21841 x 1024 418 us against 392. x'
+//    is laid out once a call, since rows that do not count have to be zeros in it.
 //  * d is rounded to bf16 before it is scaled (and divided by 1 - e): a label's entry p - 1 then rounds the
 //    same whatever the batch size, and the scale is applied to the fp32 sums. Only an upstream gradient for
 //    each row goes into d, since the sum over n cannot apply it.
@@ -33,14 +33,6 @@ using Big = GemmTile<256, 256, 2, 4>;
 using Mid = GemmTile<128, 128, 2, 2>;
 using Small = GemmTile<64, 64, 2, 2>;
 using Thin = ThinTile;
-// the tiles of dx (w read [v][k]) and of dw (d read [n][v])
-template <class T>
-struct OutTiles { using X = T; using W = T; };
-template <>
-struct OutTiles<Big> {
-  using X = GemmTile<256, 256, 2, 4, true, false>;
-  using W = GemmTile<256, 256, 2, 4, false, true>;
-};
 
 constexpr int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 constexpr int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
@@ -245,31 +237,25 @@ __global__ __launch_bounds__(256) void total_kernel(const float2* __restrict__ b
 }
 
 // --------------------------------------------------------------------------------------- backward
-// dst[c][r] = src[r][c] for r < rows (by_label: only of counted rows), 0 up to ldd; 64 x 64 by 256 threads,
-// one or two matrices a launch. 16-byte loads and stores; a column of the LDS image is gathered by 2 bytes.
+// x' [width][ldt] of the rows that count, 0 in the others and up to ldt; 64 x 64 by 256 threads. 16-byte
+// loads and stores; a column of the LDS image is gathered by 2 bytes.
 struct Transpose {
-  const u16* src;
-  int64_t ld;
-  int rows, cols;
-  u16* dst;
-  int64_t ldd;
-  int by_label;
-  int blocks;  // (ldd / 64) x ceil(cols / 64)
+  u16* to;
+  int64_t ldt;
+  int blocks;  // (ldt / 64) x ceil(width / 64)
 };
 constexpr int TRANSPOSE_LDS = 64 * 74 * 2;  // 37 banks a row: gathers of 8 rows apart do not meet
-DV_DEVICE void transpose_block(const DvXent& x, const Transpose& m0, const Transpose& m1, int id, int tid, char* smem) {
+DV_DEVICE void transpose_block(const DvXent& x, const Transpose& t, int id, int tid, char* smem) {
   u16(*sh)[74] = reinterpret_cast<u16(*)[74]>(smem);
-  const bool any = id < m0.blocks + m1.blocks;
-  const Transpose& t = id < m0.blocks ? m0 : m1;
-  if (id >= m0.blocks) id -= m0.blocks;
-  const int across = any ? (int)(t.ldd / 64) : 1, r0 = id % across * 64, c0 = id / across * 64;
+  const bool any = id < t.blocks;
+  const int across = any ? (int)(t.ldt / 64) : 1, r0 = id % across * 64, c0 = id / across * 64;
   if (any) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {  // rows of the operand hold whole 64-column blocks (zeros from `width` on)
+    for (int e = 0; e < 2; ++e) {  // rows of x hold whole 64-column blocks (zeros from `width` on)
       const int r = e * 32 + (tid >> 3), c = (tid & 7) * 8;
       uint4 d{0, 0, 0, 0};
-      if (r0 + r < t.rows && (!t.by_label || counted(x.labels[r0 + r], x)))
-        d = *reinterpret_cast<const uint4*>(t.src + (int64_t)(r0 + r) * t.ld + c0 + c);
+      if (r0 + r < x.N && counted(x.labels[r0 + r], x))
+        d = *reinterpret_cast<const uint4*>(x.x + (int64_t)(r0 + r) * x.ldx + c0 + c);
       uint32_t* to = reinterpret_cast<uint32_t*>(&sh[r][c]);
       to[0] = d.x; to[1] = d.y; to[2] = d.z; to[3] = d.w;
     }
@@ -282,32 +268,31 @@ DV_DEVICE void transpose_block(const DvXent& x, const Transpose& m0, const Trans
     uint32_t w[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) w[k] = (uint32_t)sh[r + 2 * k][c] | (uint32_t)sh[r + 2 * k + 1][c] << 16;
-    if (c0 + c < t.cols) *reinterpret_cast<uint4*>(t.dst + (int64_t)(c0 + c) * t.ldd + r0 + r) = uint4{w[0], w[1], w[2], w[3]};
+    if (c0 + c < x.width) *reinterpret_cast<uint4*>(t.to + (int64_t)(c0 + c) * t.ldt + r0 + r) = uint4{w[0], w[1], w[2], w[3]};
   }
 }
-__global__ __launch_bounds__(256) void transpose_kernel(DvXent x, Transpose m0, Transpose m1) {
+__global__ __launch_bounds__(256) void transpose_kernel(DvXent x, Transpose t) {
   __shared__ __attribute__((aligned(16))) char smem[TRANSPOSE_LDS];
-  transpose_block(x, m0, m1, blockIdx.x, threadIdx.x, smem);
+  transpose_block(x, t, blockIdx.x, threadIdx.x, smem);
 }
 
-// d (times t, where each row has a gradient of its own) of the piece [p0, p0 + pv) of the vocabulary:
-// P [n][pvp], zero from pv and from N on, and Q [v][ldq], or null; db partial sums [n block and wave][pv]
+// d (times its gradient, where each row has one of its own) of the piece [p0, p0 + pv) of the vocabulary:
+// P [ldt][pvp], zero from N and from pv on; db partial sums [n block and wave][pv]
 template <class T, int BM, int BN, int WN>
 __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(DvXent a, const float2* __restrict__ lse, int p0,
-                                                                              int pv, int pvp, u16* __restrict__ P,
-                                                                              u16* __restrict__ Q, int64_t ldq,
+                                                                              int pv, int pvp, u16* __restrict__ P, int ldt,
                                                                               float* __restrict__ pbias, int tiles,
-                                                                              Transpose m0, Transpose m1) {
+                                                                              Transpose xt) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  if ((int)blockIdx.x >= tiles) {  // the blocks behind the tiles lay out what the next launch reads
+  if ((int)blockIdx.x >= tiles) {  // the blocks behind the tiles lay out x', which the next launch reads
     const int sub = threadIdx.x >> 8;
-    transpose_block(a, m0, m1, (blockIdx.x - tiles) * (T::NTHREADS / 256) + sub, threadIdx.x & 255, smem + sub * TRANSPOSE_LDS);
+    transpose_block(a, xt, (blockIdx.x - tiles) * (T::NTHREADS / 256) + sub, threadIdx.x & 255, smem + sub * TRANSPOSE_LDS);
     return;
   }
-  constexpr int PITCH = 144;  // bytes: 64 bf16 + 16, conflict-free both ways
+  constexpr int PITCH = 144;  // bytes: 64 bf16 + 16, without bank conflicts
   constexpr int MG = T::TM < 2 ? 1 : 2, MW = 32 * MG, NW = 32 * T::TN;
-  // tiles up to pvp and ldq: where a tile is half of 64 the last one may hold nothing but zeros of P or Q
-  const int tm = (pvp + BM - 1) / BM, tn = (int)((ldq + BN - 1) / BN);
+  // tiles up to pvp and ldt: where a tile is half of 64 the last one may hold nothing but zeros
+  const int tm = (pvp + BM - 1) / BM, tn = (ldt + BN - 1) / BN;
   const TileAt at = tile_at(blockIdx.x, tiles, tm, tn);
   const int v0 = at.m * BM, n0 = at.n * BN;  // v: within the piece
   T t;
@@ -369,13 +354,11 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(Dv
         if ((t.lane & 31) == 0 && v < pv) pbias[(int64_t)(at.n * WN + t.wn) * pv + v] = s;
       }
   }
-  // both layouts through this wave's own part of LDS, MW columns of the vocabulary at a time
-  char* mine = smem + t.wave * (NW > MW ? NW : MW) * PITCH;
-  const uint32_t swap = t.lane & 1 ? 0x07060302u : 0x01000504u;
+  // rows of P through this wave's own part of LDS, MW columns of the vocabulary at a time
+  char* mine = smem + t.wave * NW * PITCH;
 #pragma unroll
   for (int h = 0; h < T::TM / MG; ++h) {
     const int vw = v0 + (t.wm * T::TM + h * MG) * 32, nw = n0 + t.wn * T::TN * 32;
-    uint32_t u[MG][T::TN][8];  // pairs of columns v of this lane's row n
 #pragma unroll
     for (int j = 0; j < T::TN; ++j)
 #pragma unroll
@@ -383,43 +366,22 @@ __global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void grad_kernel(Dv
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const f32x16& c = t.acc[h * MG + i][j];
-          u[i][j][2 * q] = pack2bf(c[4 * q], c[4 * q + 1]);
-          u[i][j][2 * q + 1] = pack2bf(c[4 * q + 2], c[4 * q + 3]);
           *reinterpret_cast<uint2*>(mine + (j * 32 + (t.lane & 31)) * PITCH + (i * 32 + 8 * q + 4 * (t.lane >> 5)) * 2) =
-              uint2{u[i][j][2 * q], u[i][j][2 * q + 1]};
+              uint2{pack2bf(c[4 * q], c[4 * q + 1]), pack2bf(c[4 * q + 2], c[4 * q + 3])};
         }
     wave_sync();
 #pragma unroll
     for (int e = 0; e < NW * MW / 512; ++e) {
       const int w = e * 64 + t.lane, n = w / (MW / 8), c = w % (MW / 8) * 8;
       const uint4 d = *reinterpret_cast<const uint4*>(mine + n * PITCH + c * 2);
-      if (nw + n < ldq && vw + c < pvp) *reinterpret_cast<uint4*>(P + (int64_t)(nw + n) * pvp + vw + c) = d;
+      if (nw + n < ldt && vw + c < pvp) *reinterpret_cast<uint4*>(P + (int64_t)(nw + n) * pvp + vw + c) = d;
     }
     wave_sync();
-    if (Q) {
-#pragma unroll
-      for (int j = 0; j < T::TN; ++j)
-#pragma unroll
-        for (int i = 0; i < MG; ++i)
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {  // columns v, v + 1 of two neighbouring rows n become rows of Q
-            const uint32_t w = u[i][j][k], o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0xB1, 0xF, 0xF, false);  // lane ^ 1
-            const int v = i * 32 + (k & 1) * 2 + 8 * (k >> 1) + 4 * (t.lane >> 5) + (t.lane & 1);
-            *reinterpret_cast<uint32_t*>(mine + v * PITCH + (j * 32 + (t.lane & 30)) * 2) = __builtin_amdgcn_perm(w, o, swap);
-          }
-      wave_sync();
-#pragma unroll
-      for (int e = 0; e < NW * MW / 512; ++e) {
-        const int w = e * 64 + t.lane, v = w / (NW / 8), c = w % (NW / 8) * 8;
-        const uint4 d = *reinterpret_cast<const uint4*>(mine + v * PITCH + c * 2);
-        if (vw + v < pv && nw + c < ldq) *reinterpret_cast<uint4*>(Q + (int64_t)(vw + v) * ldq + nw + c) = d;
-      }
-      wave_sync();
-    }
   }
 }
 
-// out[n][m] = scale * sum_k A[m][k] B[n][k] over this split's K-tiles
+// out[n][m] = scale * sum_k A[m][k] B[n][k] over this split's K-tiles. dx: A = w' and B = d; dw: A = x' and
+// B = d'. w and d are read as they lie, k by k for A and for B.
 struct OutArgs {
   const u16 *a, *b;
   int64_t lda, ldb;
@@ -429,7 +391,7 @@ struct OutArgs {
   void* out;         // [N][M], bf16 or fp32
   int out_f32, out_add;
   int by_row;        // 0 in rows n whose label does not count
-  int deep;          // valid k of `a`, where the tile reads it [k][m]
+  int deep;          // valid k
 };
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
@@ -476,7 +438,7 @@ DV_DEVICE void fold_bias(const DvXent& x, const BiasArgs& b, int block, float* s
 }
 
 // tile `id` of g
-template <class T, int BM, int BN>
+template <class T, int BM, int BN, bool DX>
 DV_DEVICE void out_tile(const DvXent& x, const OutArgs& g, int id, char* smem) {
   constexpr int PITCH = 144, NW = 32 * T::TN;
   const int tm = (g.M + BM - 1) / BM, tn = (g.N + BN - 1) / BN;
@@ -484,12 +446,12 @@ DV_DEVICE void out_tile(const DvXent& x, const OutArgs& g, int id, char* smem) {
   const TileAt at = tile_at(id - split * tiles, tiles, tm, tn);
   const int m0 = at.m * BM, n0 = at.n * BN;
   const int k0 = (int)((int64_t)g.ktiles * split / g.splits), k1 = (int)((int64_t)g.ktiles * (split + 1) / g.splits);
-  GemmOperand a{g.a + (int64_t)m0 * g.lda + k0 * 64, g.lda, g.M - m0}, b{g.b + (int64_t)n0 * g.ldb + k0 * 64, g.ldb, g.N - n0};
-  if constexpr (T::TURNED_A) a = {g.a + (int64_t)k0 * 64 * g.lda + m0, g.lda, g.M - m0, g.deep - k0 * 64};
-  if constexpr (T::TURNED_B) b = {g.b + (int64_t)k0 * 64 * g.ldb + n0, g.ldb, g.N - n0, (g.ktiles - k0) * 64};
+  const int64_t k = (int64_t)k0 * 64;
+  const int deep = g.deep - k0 * 64;
+  const GemmOperand a{g.a + (DX ? k * g.lda + m0 : m0 * g.lda + k), g.lda, g.M - m0, deep};
+  const GemmOperand b{g.b + (DX ? n0 * g.ldb + k : k * g.ldb + n0), g.ldb, g.N - n0, deep};
   T t;
   t.run(a, b, k1 - k0, smem);
-  if (!t.active()) return;
   const float common = g.slab ? 1.f : common_scale(x);
   char* mine = smem + t.wave * NW * PITCH;
 #pragma unroll
@@ -523,17 +485,14 @@ DV_DEVICE void out_tile(const DvXent& x, const OutArgs& g, int id, char* smem) {
 
 // The products behind a piece's d, and the fold of its bias gradient, in one launch: blocks [0, b0) compute
 // dx, [b0, b0 + b1) dw, the rest the bias.
-template <class T, int BM, int BN>
-__global__ __launch_bounds__(T::NTHREADS, T::NTHREADS / 256) void out_kernel(DvXent x, OutArgs gx, OutArgs gw, BiasArgs bias,
-                                                                             int b0, int b1) {
+template <int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void out_kernel(DvXent x, OutArgs gx, OutArgs gw, BiasArgs bias, int b0,
+                                                                        int b1) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  using X = typename OutTiles<T>::X;
-  using W = typename OutTiles<T>::W;
   const int id = blockIdx.x;
-  if (id >= b0 + b1) return fold_bias(x, bias, id - b0 - b1, reinterpret_cast<float*>(smem));
-  if constexpr (std::is_same_v<X, W>) out_tile<T, BM, BN>(x, id < b0 ? gx : gw, id < b0 ? id : id - b0, smem);
-  else if (id < b0) out_tile<X, BM, BN>(x, gx, id, smem);
-  else out_tile<W, BM, BN>(x, gw, id - b0, smem);
+  if (id < b0) out_tile<GemmTile<BM, BN, WM, WN, true, false>, BM, BN, true>(x, gx, id, smem);
+  else if (id < b0 + b1) out_tile<GemmTile<BM, BN, WM, WN, false, true>, BM, BN, false>(x, gw, id - b0, smem);
+  else fold_bias(x, bias, id - b0 - b1, reinterpret_cast<float*>(smem));
 }
 
 // out[n][m] = scale * sum over splits of the slab
@@ -601,7 +560,7 @@ __global__ __launch_bounds__(256) void pack_kernel(DvPack m0, DvPack m1, int b0)
 // 1 .. 4096 rows, 100 .. 50000 classes and widths of 256 and 2048 the form it takes is within 13 % of the
 // best of the four, most often within 3 %.
 struct Plan { int form, splits; double us; };
-constexpr int FORMS = 4, FORM_M[FORMS] = {256, 128, 64, 32}, FORM_N[FORMS] = {256, 128, 64, 32};
+constexpr int FORMS = 4, OUT_FORMS = 3, FORM_M[FORMS] = {256, 128, 64, 32}, FORM_N[FORMS] = {256, 128, 64, 32};
 enum Ends { PLAIN, GRAD };  // what a block does behind its sums: GRAD writes both layouts of d
 Plan plan_form(int f, int64_t M, int64_t N, int ktiles, bool may_split, Ends ends) {
   // us a K-tile: on a CU with as many blocks as fit (AT_ONCE), and alone; us of a block's two ends
@@ -629,15 +588,19 @@ Plan plan(int64_t M, int64_t N, int ktiles, Ends ends) {
   return best;
 }
 
-// f(tile, BM, BN, WM, WN)
+// f(tile, BM, BN, WM, WN); the products behind d take the first three
 template <int V>
 using Int = std::integral_constant<int, V>;
 template <class F>
-void with_tile(int form, F&& f) {
+void with_wide_tile(int form, F&& f) {
   if (form == 0) f(Big{}, Int<256>{}, Int<256>{}, Int<2>{}, Int<4>{});
   else if (form == 1) f(Mid{}, Int<128>{}, Int<128>{}, Int<2>{}, Int<2>{});
-  else if (form == 2) f(Small{}, Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{});
-  else f(Thin{}, Int<32>{}, Int<32>{}, Int<1>{}, Int<1>{});
+  else f(Small{}, Int<64>{}, Int<64>{}, Int<2>{}, Int<2>{});
+}
+template <class F>
+void with_tile(int form, F&& f) {
+  if (form == 3) f(Thin{}, Int<32>{}, Int<32>{}, Int<1>{}, Int<1>{});
+  else with_wide_tile(form, f);
 }
 constexpr int FORM_WM[FORMS] = {2, 2, 2, 1}, FORM_WN[FORMS] = {4, 2, 2, 1};
 
@@ -671,48 +634,33 @@ FwdLayout fwd_layout(const DvXent& a) {
 struct BwdLayout {
   int piece;           // columns of the vocabulary at a time
   Plan pg, px, pw;     // the logits again, dx, dw
-  bool direct;         // the products read w [v][k] and d [n][v]: no w', no second layout of d
-  int64_t ldq;
+  int ldt;             // rows rounded up to 64
   int bias_parts;
   bool dx_slab;
-  int64_t P, Q, xt, wt, sx, sw, pb, bytes;
+  int64_t P, xt, sx, sw, pb, bytes;
 };
-constexpr int64_t PIECE_BYTES = 1LL << 30;  // a piece's d, in the layouts that are written
-BwdLayout bwd_layout(const DvXent& a, bool need_x, bool need_w, bool need_b, bool have_wt) {
+constexpr int64_t PIECE_BYTES = 1LL << 30;  // a piece's d
+BwdLayout bwd_layout(const DvXent& a, bool need_x, bool need_w, bool need_b) {
   BwdLayout l;
-  l.ldq = up(a.N, 64);
-  int pieces = 1;
-  auto cut = [&](int layouts) {
-    const int64_t most = std::max<int64_t>(PIECE_BYTES / (2 * layouts * l.ldq) / 256 * 256, 256);
-    pieces = cdiv(a.V, most);
-    l.piece = (int)std::min<int64_t>(up(cdiv(a.V, pieces), 256), a.V);
-  };
-  auto dx_plan = [&](int f) { return plan_form(f, a.width, a.N, cdiv(l.piece, 64), true, PLAIN); };
-  auto dw_plan = [&](int f) { return plan_form(f, a.width, l.piece, cdiv(a.N, 64), true, PLAIN); };
+  l.ldt = (int)up(a.N, 64);
+  const int64_t most = std::max<int64_t>(PIECE_BYTES / (2 * l.ldt) / 256 * 256, 256);
+  const int pieces = cdiv(a.V, most);
+  l.piece = (int)std::min<int64_t>(up(cdiv(a.V, pieces), 256), a.V);
+  l.pg = plan(l.piece, a.N, a.D / 64, GRAD);
   // dx and dw run in one launch and share a tile form, whichever of them is wanted: a gradient's bits do
   // not depend on which others are asked for
-  cut(2);
   double least = 1e30;
-  for (int f = 0; f < FORMS; ++f) {
-    const Plan x = dx_plan(f), w = dw_plan(f);
+  for (int f = 0; f < OUT_FORMS; ++f) {
+    const Plan x = plan_form(f, a.width, a.N, cdiv(l.piece, 64), true, PLAIN),
+               w = plan_form(f, a.width, l.piece, cdiv(a.N, 64), true, PLAIN);
     if (x.us + w.us < least) { least = x.us + w.us; l.px = x; l.pw = w; }
   }
-  l.direct = l.px.form == 0;
-  if (l.direct) {
-    cut(1);
-    l.px = dx_plan(0);
-    l.pw = dw_plan(0);
-  }
-  l.pg = plan(l.piece, a.N, a.D / 64, GRAD);
-  l.bias_parts = cdiv(l.ldq, FORM_N[l.pg.form]) * FORM_WN[l.pg.form];
+  l.bias_parts = cdiv(l.ldt, FORM_N[l.pg.form]) * FORM_WN[l.pg.form];
   l.dx_slab = l.px.splits > 1 || pieces > 1;
-  const int64_t pvp = up(l.piece, 64);
   int64_t at = 0;
   auto take = [&](int64_t b) { const int64_t o = at; at += up(b, 256); return o; };
-  l.P = take(l.ldq * pvp * 2);
-  l.Q = take(need_w && !l.direct ? (int64_t)l.piece * l.ldq * 2 : 0);
-  l.xt = take(need_w ? (int64_t)a.width * l.ldq * 2 : 0);
-  l.wt = take(need_x && !have_wt && !l.direct ? (int64_t)a.width * pvp * 2 : 0);
+  l.P = take(l.ldt * up(l.piece, 64) * 2);
+  l.xt = take(need_w ? (int64_t)a.width * l.ldt * 2 : 0);
   l.sx = take(need_x && l.dx_slab ? (int64_t)l.px.splits * a.N * a.width * 4 : 0);
   l.sw = take(need_w && l.pw.splits > 1 ? (int64_t)l.pw.splits * l.piece * a.width * 4 : 0);
   l.pb = take(need_b ? (int64_t)l.bias_parts * l.piece * 4 : 0);
@@ -727,16 +675,16 @@ bool sane(const DvXent& a) {
          ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0;
 }
 
-void launch_out(const DvXent& a, int form, const OutArgs& g0, const OutArgs& g1, const BiasArgs& bias, hipStream_t st) {
-  with_tile(form, [&](auto tile, auto bm, auto bn, auto, auto) {
+void launch_out(const DvXent& a, int form, const OutArgs& gx, const OutArgs& gw, const BiasArgs& bias, hipStream_t st) {
+  with_wide_tile(form, [&](auto tile, auto bm, auto bn, auto wm, auto wn) {
     using T = decltype(tile);
-    constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value;
-    const int b0 = cdiv(g0.M, BM) * cdiv(g0.N, BN) * g0.splits, b1 = cdiv(g1.M, BM) * cdiv(g1.N, BN) * g1.splits;
+    constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
+    const int b0 = cdiv(gx.M, BM) * cdiv(gx.N, BN) * gx.splits, b1 = cdiv(gw.M, BM) * cdiv(gw.N, BN) * gw.splits;
     const int b2 = bias.db ? cdiv(bias.pv, 64) : 0;
     if (b0 + b1 + b2 == 0) return;
     static bool done[64];
-    allow_lds(out_kernel<T, BM, BN>, T::LDS, done);
-    out_kernel<T, BM, BN><<<(unsigned)(b0 + b1 + b2), T::NTHREADS, T::LDS, st>>>(a, g0, g1, bias, b0, b1);
+    allow_lds(out_kernel<BM, BN, WM, WN>, T::LDS, done);
+    out_kernel<BM, BN, WM, WN><<<(unsigned)(b0 + b1 + b2), T::NTHREADS, T::LDS, st>>>(a, gx, gw, bias, b0, b1);
   });
 }
 void launch_reduce(const DvXent& a, const OutArgs& g, hipStream_t st) {
@@ -746,11 +694,9 @@ void launch_reduce(const DvXent& a, const OutArgs& g, hipStream_t st) {
 }  // namespace
 
 int64_t dv_linear_xent_fwd_bytes(const DvXent& a) { return fwd_layout(a).bytes; }
-int64_t dv_linear_xent_bwd_bytes(const DvXent& a, int need_x, int need_w, int need_b, int have_wt) {
-  return bwd_layout(a, need_x, need_w, need_b, have_wt).bytes;
+int64_t dv_linear_xent_bwd_bytes(const DvXent& a, int need_x, int need_w, int need_b) {
+  return bwd_layout(a, need_x, need_w, need_b).bytes;
 }
-
-int dv_linear_xent_reads_wt(const DvXent& a) { return !bwd_layout(a, true, true, true, true).direct; }
 
 int dv_linear_xent_fwd(const DvXent& a, void* ws, float* lse, float* loss_rows, float* total, float* out, hipStream_t st) {
   if (!sane(a)) return -1;
@@ -775,50 +721,38 @@ int dv_linear_xent_fwd(const DvXent& a, void* ws, float* lse, float* loss_rows, 
   return 0;
 }
 
-int dv_linear_xent_bwd(const DvXent& a, void* ws, const float* lse, const void* wt_all, int64_t ldwt, void* dx, void* dw,
-                       int dw_f32, int dw_add, float* db, int db_add, hipStream_t st) {
+int dv_linear_xent_bwd(const DvXent& a, void* ws, const float* lse, void* dx, void* dw, int dw_f32, int dw_add, float* db,
+                       int db_add, hipStream_t st) {
   if (!sane(a)) return -1;
   const bool need_w = dw != nullptr, need_x = dx != nullptr;
-  const BwdLayout l = bwd_layout(a, need_x, need_w, db != nullptr, wt_all != nullptr);
+  const BwdLayout l = bwd_layout(a, need_x, need_w, db != nullptr);
   char* w = reinterpret_cast<char*>(ws);
-  u16 *P = reinterpret_cast<u16*>(w + l.P), *Q = need_w && !l.direct ? reinterpret_cast<u16*>(w + l.Q) : nullptr;
-  u16 *xt = reinterpret_cast<u16*>(w + l.xt), *wt = reinterpret_cast<u16*>(w + l.wt);
+  u16 *P = reinterpret_cast<u16*>(w + l.P), *xt = reinterpret_cast<u16*>(w + l.xt);
   float* pb = db ? reinterpret_cast<float*>(w + l.pb) : nullptr;
-  auto transposed = [&](const u16* src, int64_t ld, int rows, u16* dst, int64_t ldd, int by_label) {
-    return Transpose{src, ld, rows, a.width, dst, ldd, by_label, (int)(ldd / 64) * cdiv(a.width, 64)};
-  };
   OutArgs gx{};
   for (int p0 = 0; p0 < a.V; p0 += l.piece) {
     const int pv = std::min(l.piece, a.V - p0), pvp = (int)up(pv, 64);
-    Transpose tx{}, tw{};
-    if (need_w && p0 == 0) tx = transposed(a.x, a.ldx, a.N, xt, l.ldq, 1);
-    if (need_x && !wt_all && !l.direct) tw = transposed(a.w + (int64_t)p0 * a.ldw, a.ldw, pv, wt, pvp, 0);
+    const Transpose tx{xt, l.ldt, need_w && p0 == 0 ? l.ldt / 64 * cdiv(a.width, 64) : 0};
     // in the gradient's launch, but for the largest tiles: a block there takes a CU's LDS, whatever it does
-    // (8192 x 65536 x 2048: 50 us apart, 80 rounds of blocks within)
-    int beside = tx.blocks + tw.blocks;
-    if (beside && l.pg.form == 0) {
-      transpose_kernel<<<(unsigned)beside, 256, 0, st>>>(a, tx, tw);
-      beside = 0;
-    }
+    const bool apart = l.pg.form == 0;
+    if (apart && tx.blocks) transpose_kernel<<<(unsigned)tx.blocks, 256, 0, st>>>(a, tx);
     with_tile(l.pg.form, [&](auto tile, auto bm, auto bn, auto, auto wn) {
       using T = decltype(tile);
       constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WN = decltype(wn)::value;
       static bool done[64];
       allow_lds(grad_kernel<T, BM, BN, WN>, T::LDS, done);
-      const int tiles = cdiv(pvp, BM) * cdiv(l.ldq, BN), more = cdiv(beside, T::NTHREADS / 256);
-      grad_kernel<T, BM, BN, WN><<<(unsigned)(tiles + more), T::NTHREADS, T::LDS, st>>>(
-          a, reinterpret_cast<const float2*>(lse), p0, pv, pvp, P, Q, l.ldq, pb, tiles, tx, tw);
+      const int tiles = cdiv(pvp, BM) * cdiv(l.ldt, BN), beside = apart ? 0 : cdiv(tx.blocks, T::NTHREADS / 256);
+      grad_kernel<T, BM, BN, WN><<<(unsigned)(tiles + beside), T::NTHREADS, T::LDS, st>>>(
+          a, reinterpret_cast<const float2*>(lse), p0, pv, pvp, P, l.ldt, pb, tiles, tx);
     });
     OutArgs gw{};
-    if (need_x) {
-      const u16* rows = l.direct ? a.w + (int64_t)p0 * a.ldw : wt_all ? reinterpret_cast<const u16*>(wt_all) + p0 : wt;
-      gx = OutArgs{rows, P, l.direct ? a.ldw : wt_all ? ldwt : pvp, pvp, a.width, a.N, pvp / 64, std::min(l.px.splits, pvp / 64),
+    if (need_x)
+      gx = OutArgs{a.w + (int64_t)p0 * a.ldw, P, a.ldw, pvp, a.width, a.N, pvp / 64, std::min(l.px.splits, pvp / 64),
                    l.dx_slab ? reinterpret_cast<float*>(w + l.sx) : nullptr, p0 > 0, dx, 0, 0, 1, pv};
-    }
     if (need_w) {
       char* to = reinterpret_cast<char*>(dw) + (int64_t)p0 * a.width * (dw_f32 ? 4 : 2);
-      gw = OutArgs{xt, l.direct ? P : Q, l.ldq, l.direct ? pvp : l.ldq, a.width, pv, (int)(l.ldq / 64), l.pw.splits,
-                   l.pw.splits > 1 ? reinterpret_cast<float*>(w + l.sw) : nullptr, 0, to, dw_f32, dw_add, 0, 0};
+      gw = OutArgs{xt, P, l.ldt, pvp, a.width, pv, l.ldt / 64, l.pw.splits,
+                   l.pw.splits > 1 ? reinterpret_cast<float*>(w + l.sw) : nullptr, 0, to, dw_f32, dw_add, 0, l.ldt};
     }
     const BiasArgs gb{pb, l.bias_parts, pv, db ? db + p0 : nullptr, db_add};
     launch_out(a, l.px.form, gx, gw, gb, st);

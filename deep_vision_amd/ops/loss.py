@@ -97,7 +97,7 @@ def _operands(x, weight, D, Dp):
 
 
 def _cached_weight(weight):
-    """fp32 parameters keep their bf16 operands from step to step (ops/wcache.py)."""
+    """fp32 parameters keep their bf16 operand from step to step (ops/wcache.py)."""
     return weight.dtype == F32 and isinstance(weight, torch.nn.Parameter) and weight.is_contiguous()
 
 
@@ -106,13 +106,6 @@ def _operand(weight, Dp):
 
     V, D = weight.shape
     return _prep_weight(weight.view(V, D, 1, 1), 1, Dp, mode=0, param=weight).view(V, Dp)
-
-
-def _transposed_operand(weight, Vp):
-    from .conv import _prep_weight
-
-    V, D = weight.shape
-    return _prep_weight(weight.view(V, D, 1, 1), 1, Vp, mode=1, param=weight)
 
 
 def _linear_xent_args(xk, wk, b, labels, V, Dp, D, ignore_index, smoothing, reduction):
@@ -173,17 +166,12 @@ def _linear_xent_backward(ctx, go, sinks):
     if go.dtype != F32 or not go.is_contiguous():
         go = go.to(F32).contiguous()
     # (the engine runs a node on the device and stream of its forward pass)
-    wt, Vp = None, (V + 63) // 64 * 64
-    cached = wk is None
-    if cached:  # the parameter's operands, as they are now
+    if wk is None:  # the parameter's operand, as it is now
         wk = _operand(weight, Dp)
     args = _linear_xent_args(xk, wk, b, labels, V, Dp, D, ignore_index, smoothing, reduction)
-    if cached and need_x and Vp <= 1 << 22 and lib().linear_xent_reads_wt(*args):
-        wt = _transposed_operand(weight, Vp)
-    ws = x.new_empty(lib().linear_xent_bwd_bytes(*args, int(need_x), int(need_w), int(need_b), int(wt is not None)),
-                     dtype=torch.uint8)
+    ws = x.new_empty(lib().linear_xent_bwd_bytes(*args, int(need_x), int(need_w), int(need_b)), dtype=torch.uint8)
     at = stats.data_ptr()
-    lib().linear_xent_bwd(*args, ptr(go), at + 8 * N, ptr(ws), at, ptr(wt), Vp, ptr(dx), ptr(dw),
+    lib().linear_xent_bwd(*args, ptr(go), at + 8 * N, ptr(ws), at, ptr(dx), ptr(dw),
                           int(weight.dtype == F32), int(sw is not None), ptr(db), int(sb is not None), stream_handle())
     return dx, None if sw is not None else dw, None if sb is not None else db, None, None, None, None
 
