@@ -557,15 +557,15 @@ __global__ __launch_bounds__(256) void pack_kernel(DvPack m0, DvPack m1, int b0)
 // ------------------------------------------------------------------------------------------- host
 // Tile and split of an M x N x (64 ktiles) product: the least time by a model of a K-tile's time on a full
 // CU (throughput) and alone (latency) and of a block's ends, its constants fitted to measurements. Over
-// 1 .. 4096 rows, 100 .. 50000 classes and widths of 256 and 2048 the form it takes is within 13 % of the
-// best of the four, most often within 3 %.
+// 1 .. 8192 rows, 64 .. 65536 classes and widths of 64 .. 2500 (88 shapes) the form it takes is within 13 % of
+// the best, within 3 % for nine in ten.
 struct Plan { int form, splits; double us; };
 constexpr int FORMS = 4, OUT_FORMS = 3, FORM_M[FORMS] = {256, 128, 64, 32}, FORM_N[FORMS] = {256, 128, 64, 32};
-enum Ends { PLAIN, GRAD };  // what a block does behind its sums: GRAD writes both layouts of d
+enum Ends { STATS, GRAD, OUT };  // what a block does behind its sums
 Plan plan_form(int f, int64_t M, int64_t N, int ktiles, bool may_split, Ends ends) {
   // us a K-tile: on a CU with as many blocks as fit (AT_ONCE), and alone; us of a block's two ends
   constexpr double FULL[FORMS] = {1.6, 0.58, 0.25, 0.2}, ALONE[FORMS] = {1.6, 0.65, 0.35, 0.2};
-  constexpr double ENDS[2][FORMS] = {{4, 2.5, 2, 2.5}, {16, 9, 4, 5}};
+  constexpr double ENDS[3][FORMS] = {{4, 2.5, 2, 2.5}, {16, 9, 4, 5}, {6, 2.5, 1}};
   constexpr int AT_ONCE[FORMS] = {1, 2, 5, 2};
   Plan best{f, 1, 1e30};
   const int64_t tiles = (int64_t)cdiv(M, FORM_M[f]) * cdiv(N, FORM_N[f]);
@@ -617,7 +617,7 @@ void allow_lds(K kernel, int bytes, bool (&done)[64]) {
 struct FwdLayout { Plan p; int parts, rows, blocks; int64_t part, psum, label, block, bytes; };
 FwdLayout fwd_layout(const DvXent& a) {
   FwdLayout l;
-  l.p = plan(a.V, a.N, a.D / 64, PLAIN);
+  l.p = plan(a.V, a.N, a.D / 64, STATS);
   l.parts = cdiv(a.V, FORM_M[l.p.form]) * FORM_WM[l.p.form];
   l.rows = a.N <= 256 && l.parts <= 128 ? 256 : 16;  // small: one block joins every row
   l.blocks = cdiv(a.N, l.rows);
@@ -651,8 +651,8 @@ BwdLayout bwd_layout(const DvXent& a, bool need_x, bool need_w, bool need_b) {
   // not depend on which others are asked for
   double least = 1e30;
   for (int f = 0; f < OUT_FORMS; ++f) {
-    const Plan x = plan_form(f, a.width, a.N, cdiv(l.piece, 64), true, PLAIN),
-               w = plan_form(f, a.width, l.piece, cdiv(a.N, 64), true, PLAIN);
+    const Plan x = plan_form(f, a.width, a.N, cdiv(l.piece, 64), true, OUT),
+               w = plan_form(f, a.width, l.piece, cdiv(a.N, 64), true, OUT);
     if (x.us + w.us < least) { least = x.us + w.us; l.px = x; l.pw = w; }
   }
   l.bias_parts = cdiv(l.ldt, FORM_N[l.pg.form]) * FORM_WN[l.pg.form];
