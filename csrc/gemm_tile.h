@@ -86,7 +86,8 @@ struct GemmTile {
     const int k = (lane & 15) >> 2;
 #pragma unroll
     for (int i = 0; i < I; ++i) {
-      if constexpr (K) at[i] = ((lane >> 5) * 8 + k) * B * 2 + (((w * T + i) ^ unit_swizzle<B>(k)) << 6) + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+      if constexpr (K)
+        at[i] = ((lane >> 5) * 8 + k) * B * 2 + (((w * T + i) ^ unit_swizzle<B>(k)) << 6) + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
       else at[i] = (w * T * 32 + (lane & 31)) * 128;
     }
   }
@@ -95,7 +96,8 @@ struct GemmTile {
   static DV_DEVICE bf16x8 turned(char* at) {
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     using Lds = __attribute__((address_space(3))) s16x4*;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)at), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at + 4 * B * 2));
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)at);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(at + 4 * B * 2));
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 

@@ -182,8 +182,8 @@ def grad_sink(param):
 
 def accumulation_sink(ctx, index, param):
     """``grad_sink(param)`` where this backward pass is going to add the gradient of the ``index``-th
-    tensor among the function's inputs (None is not one) to ``param.grad``; None under ``torch.autograd.grad`` (which wants the gradient returned and
-    ``.grad`` untouched), for a pass that leaves the parameter out, and where the parameter has
+    tensor among the function's inputs (None is not one) to ``param.grad``; None under
+    ``torch.autograd.grad`` (which wants the gradient returned and ``.grad`` untouched), for a pass that leaves the parameter out, and where the parameter has
     hooks that read its gradient."""
     sink = grad_sink(param)
     if sink is None or param._backward_hooks:

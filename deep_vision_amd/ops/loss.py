@@ -139,9 +139,9 @@ def _linear_xent_forward(x, weight, bias, labels, smoothing, ignore_index, reduc
 
 class _LinearXentFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, labels, smoothing, ignore_index, reduction):
+    def forward(ctx, x, weight, bias, labels, smoothing, ignore_index, reduction, leaf):  # leaf: the caller's x
         with on_device(x):
-            track_leaves(ctx, x, weight, bias)
+            track_leaves(ctx, *leaf, weight, bias)
             loss, saved = _linear_xent_forward(x, weight, bias, labels, smoothing, ignore_index, reduction, True)
         ctx.cfg = (smoothing, ignore_index, reduction)
         ctx.save_for_backward(x, weight, bias, *saved)
@@ -173,7 +173,7 @@ def _linear_xent_backward(ctx, go, sinks):
     at = stats.data_ptr()
     lib().linear_xent_bwd(*args, ptr(go), at + 8 * N, ptr(ws), at, ptr(dx), ptr(dw),
                           int(weight.dtype == F32), int(sw is not None), ptr(db), int(sb is not None), stream_handle())
-    return dx, None if sw is not None else dw, None if sb is not None else db, None, None, None, None
+    return dx, None if sw is not None else dw, None if sb is not None else db, None, None, None, None, None
 
 
 _apply_linear_xent = fast_apply(_LinearXentFn)
@@ -227,7 +227,7 @@ def linear_cross_entropy(x, weight, labels, bias=None, label_smoothing=0.0, igno
         x2 = x2.to(BF16)
     args = (x2, weight, bias, flat if flat.is_contiguous() else flat.contiguous(), float(label_smoothing), int(ignore_index), code)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, weight, bias)):
-        loss = _apply_linear_xent(*args)
+        loss = _apply_linear_xent(*args, (x,))
     else:
         with on_device(x):
             loss = _linear_xent_forward(x2, weight, bias, *args[3:], False)[0]

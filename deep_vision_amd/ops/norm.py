@@ -45,9 +45,9 @@ def _forward(x, ld, weight, bias, eps, train):
 
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps):
+    def forward(ctx, x, weight, bias, eps, leaves):  # leaves: the caller's tensors, whose views the others may be
         with on_device(x):
-            track_leaves(ctx, x, weight, bias)
+            track_leaves(ctx, *leaves)
             x2, ld = _rows(x, x.shape[-1])
             y, stats = _forward(x2, ld, _dense(weight), _dense(bias), eps, True)
         ctx.save_for_backward(x, weight, bias, stats)
@@ -61,13 +61,13 @@ class _LayerNormFn(torch.autograd.Function):
 def _backward(ctx, dy, sinks):
     # runs on autograd's device thread, where every Python step costs more than in the forward pass
     x, weight, bias, stats = ctx.saved_tensors
-    need_x, need_w, need_b, _ = ctx.needs_input_grad
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
     dtype = x.dtype
     dx = (torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=dtype, device=x.device)) if need_x else None
     x, ld = _rows(x, x.shape[-1])
     rows, D = x.shape
     if not rows:
-        return dx, torch.zeros_like(weight) if need_w else None, torch.zeros_like(bias) if need_b else None, None
+        return dx, torch.zeros_like(weight) if need_w else None, torch.zeros_like(bias) if need_b else None, None, None
     g, ldg = _rows(dy if dy.dtype == dtype else dy.to(dtype), D)
     w = _dense(weight)
     sw = accumulation_sink(ctx, 1, weight) if need_w and sinks else None
@@ -80,7 +80,7 @@ def _backward(ctx, dy, sinks):
     # (the engine runs a node on the device and stream of its forward pass)
     lib().layer_norm_bwd(x.data_ptr(), bf16, ld, g.data_ptr(), ldg, ptr(w), stats.data_ptr(), ptr(dx), ptr(part), parts, ptr(dw),
                          ptr(db), int(sw is not None), int(sb is not None), rows, D, stream_handle())
-    return dx, None if sw is not None else dw, None if sb is not None else db, None
+    return dx, None if sw is not None else dw, None if sb is not None else db, None, None
 
 
 _apply = fast_apply(_LayerNormFn)
@@ -121,8 +121,9 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
             x2, ld = _rows(x, D)
             y = _forward(x2, ld, _dense(weight), _dense(bias), float(eps), False)[0]
         return y if x.dim() == 2 and lead == 1 else y.view(x.shape)
+    leaves = (x, weight, bias)
     if len(shape) > 1:
         x2 = x.reshape(*x.shape[:-len(shape)], D)
         weight, bias = (t.reshape(D) if t is not None else None for t in (weight, bias))
-        return _apply(x2, weight, bias, float(eps)).reshape(x.shape)
-    return _apply(x, weight, bias, float(eps))
+        return _apply(x2, weight, bias, float(eps), leaves).reshape(x.shape)
+    return _apply(x, weight, bias, float(eps), leaves)

@@ -109,6 +109,37 @@ def test_cpu_matches_torch():
     assert list(m.state_dict()) == ["weight", "bias"]
 
 
+@pytest.mark.parametrize("op", ["layer_norm", "linear_cross_entropy"])
+def test_capture_is_refused_for_leaves_behind_a_view_or_a_cast(monkeypatch, op):
+    """The ops reshape and cast what they are given: the leaves that count are the caller's."""
+    from deep_vision_amd.ops import common, loss, norm
+
+    now = {"stream": 1, "capturing": False}
+    monkeypatch.setattr(common, "stream_handle", lambda: now["stream"])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now["capturing"])
+    for m in (norm, loss):
+        monkeypatch.setattr(m, "native", lambda x: True)
+    monkeypatch.setattr(norm, "_forward", lambda x, ld, w, b, eps, train: (x * 1, None))
+    monkeypatch.setattr(loss, "_linear_xent_forward", lambda x, w, b, y, *a: (x.float().sum(), (y, x, w, b, None)))
+    x = torch.randn(3, 2, 8)
+    if op == "layer_norm":
+        w, b = torch.ones(2, 8), torch.zeros(2, 8)
+        leaves, call = (x, w, b), lambda: norm.layer_norm(x, (2, 8), w, b)
+    else:
+        w, y = torch.randn(5, 8).to(torch.bfloat16), torch.zeros(3, 2, dtype=torch.int64)
+        leaves, call = (x, w), lambda: loss.linear_cross_entropy(x, w, y)
+    for leaf in leaves:
+        leaf.requires_grad_()
+        now.update(stream=1, capturing=False)
+        alive = call()
+        now.update(stream=2, capturing=True)
+        with pytest.raises(RuntimeError, match="still alive"):
+            call()
+        del alive
+        call()
+        leaf.requires_grad_(False)
+
+
 def test_capture_is_refused_while_an_eager_graph_lives(monkeypatch):
     """The bookkeeping of track_leaves on the CPU: another stream's live graph of the same leaf."""
     from deep_vision_amd.ops import common
