@@ -183,10 +183,15 @@ def grad_sink(param):
 def accumulation_sink(ctx, index, param):
     """``grad_sink(param)`` where this backward pass is going to add the gradient of the ``index``-th
     tensor among the function's inputs (None is not one) to ``param.grad``; None under
-    ``torch.autograd.grad`` (which wants the gradient returned and ``.grad`` untouched), for a pass that leaves the parameter out, and where the parameter has
-    hooks that read its gradient."""
+    ``torch.autograd.grad`` (which wants the gradient returned and ``.grad`` untouched), for a pass
+    that leaves the parameter out, where the parameter has hooks that read its gradient, and where
+    a graph built on another stream is alive: the gradient's accumulation then belongs to that
+    stream, which the engine makes wait for a returned gradient only."""
     sink = grad_sink(param)
     if sink is None or param._backward_hooks:
+        return None
+    stream = stream_handle()
+    if any(e[2] != stream and e[0]() is not None and e[1]() is param for e in _GRAPHS.get(id(param), ())):
         return None
     try:
         return sink if torch._C._will_engine_execute_node(ctx.next_functions[index][0]) else None

@@ -140,6 +140,41 @@ def test_capture_is_refused_for_leaves_behind_a_view_or_a_cast(monkeypatch, op):
         leaf.requires_grad_(False)
 
 
+def test_no_sink_while_a_graph_of_another_stream_lives(monkeypatch):
+    """The accumulation node would belong to the other stream, which nothing orders behind an in-place sum."""
+    from deep_vision_amd.ops import common
+
+    now = {"stream": 1}
+    monkeypatch.setattr(common, "stream_handle", lambda: now["stream"])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    sank = []
+
+    class Fn(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, w):
+            common.track_leaves(ctx, w)
+            ctx.save_for_backward(w)
+            return w * 2
+
+        @staticmethod
+        def backward(ctx, g):
+            sink = common.accumulation_sink(ctx, 0, ctx.saved_tensors[0])
+            sank.append(sink is not None)
+            if sink is None:
+                return g * 2
+            sink.add_(g * 2)
+
+    w = torch.nn.Parameter(torch.ones(3))
+    w.grad = torch.zeros(3)
+    Fn.apply(w).sum().backward()
+    kept = Fn.apply(w)
+    now["stream"] = 2
+    Fn.apply(w).sum().backward()
+    del kept
+    Fn.apply(w).sum().backward()
+    assert sank == [True, False, True] and torch.equal(w.grad, torch.full((3,), 6.0))
+
+
 def test_capture_is_refused_while_an_eager_graph_lives(monkeypatch):
     """The bookkeeping of track_leaves on the CPU: another stream's live graph of the same leaf."""
     from deep_vision_amd.ops import common
