@@ -161,19 +161,21 @@ __global__ __launch_bounds__(1024) void join_kernel(DvXent a, const float2* __re
                                                     float2* __restrict__ lse, float* __restrict__ loss,
                                                     float2* __restrict__ blocks, float* __restrict__ out,
                                                     float* __restrict__ total) {
-  constexpr int STRIPS = 1024 / ROWS;
-  __shared__ float sh[3][STRIPS][ROWS];
+  constexpr int STRIPS = 1024 / ROWS, GROUPS = ROWS < 64 ? 16 : STRIPS;  // a wave joins its own strips first
+  __shared__ float sh[3][GROUPS][ROWS];
   __shared__ float red[2][ROWS < 64 ? 1 : ROWS / 64];
-  const int j = threadIdx.x % ROWS, k = threadIdx.x / ROWS;
+  const int j = threadIdx.x % ROWS, k = threadIdx.x / ROWS, group = ROWS < 64 ? threadIdx.x >> 6 : k;
   const int64_t n = (int64_t)blockIdx.x * ROWS + j;
   float top = -INFINITY;
   if (n < a.N)
 #pragma unroll 8
     for (int p = k; p < parts; p += STRIPS) top = fmaxf(top, part[(int64_t)p * a.N + n].x);
-  sh[0][k][j] = top;
+#pragma unroll
+  for (int o = ROWS; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  sh[0][group][j] = top;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < STRIPS; ++i) top = fmaxf(top, sh[0][i][j]);
+  for (int i = 0; i < GROUPS; ++i) top = fmaxf(top, sh[0][i][j]);
   float s = 0.f, sum = 0.f;  // of exp(l - top), of l - top
   if (n < a.N)
 #pragma unroll 8
@@ -185,14 +187,19 @@ __global__ __launch_bounds__(1024) void join_kernel(DvXent a, const float2* __re
         if (cols > 0) sum += psum[(int64_t)p * a.N + n] + (q.x == -INFINITY ? 0.f : cols * (q.x - top));
       }
     }
-  sh[1][k][j] = s;
-  sh[2][k][j] = sum;
+#pragma unroll
+  for (int o = ROWS; o < 64; o <<= 1) {
+    s += __shfl_xor(s, o, 64);
+    sum += __shfl_xor(sum, o, 64);
+  }
+  sh[1][group][j] = s;
+  sh[2][group][j] = sum;
   __syncthreads();
   float l = 0.f, one = 0.f;
   if (k == 0) {
     float tot = 0.f, all = 0.f;
 #pragma unroll
-    for (int i = 0; i < STRIPS; ++i) { tot += sh[1][i][j]; all += sh[2][i][j]; }
+    for (int i = 0; i < GROUPS; ++i) { tot += sh[1][i][j]; all += sh[2][i][j]; }
     if (n < a.N) {
       if (counted(a.labels[n], a)) {
         one = 1.f;
