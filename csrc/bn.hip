@@ -545,12 +545,15 @@ __global__ __launch_bounds__(NT) void bn_bwd_eval_kernel(const u16* __restrict__
 inline int vec_for(int C) { return (C % 8 == 0) ? 8 : (C % 4 == 0) ? 4 : (C % 2 == 0) ? 2 : 1; }
 int g_reduce_blocks = 1024;  // benchmarking override (dv_bn_tuning)
 int g_reduce_unroll = 2;
-// (row blocks, channel slabs): ~4 blocks per CU (8 with several slabs), >= 32 rows per block
+// (row blocks, channel slabs): ~4 blocks per CU (8 with several slabs), >= 32 rows per block. Below 8192 rows
+// at most two blocks a shard: their order then does not matter (0 + a + b == 0 + b + a), so small layers'
+// sums repeat bit for bit; a third adder turned single bf16 values of dx over from run to run.
 inline dim3 reduce_grid(int64_t rows, int C) {
   const int v = vec_for(C), cg = C / v, tpr = cg < SLAB_TPR ? cg : SLAB_TPR;
   const int slabs = (cg + tpr - 1) / tpr;
   const int64_t target = (int64_t)g_reduce_blocks * (slabs > 1 ? 2 : 1) / slabs;
-  const int64_t g = std::min<int64_t>(std::max<int64_t>(target, 1), std::max<int64_t>(1, rows / 32));
+  const int64_t most = rows < 8192 ? std::min<int64_t>(rows / 32, 2 * SHARDS) : rows / 32;
+  const int64_t g = std::min<int64_t>(std::max<int64_t>(target, 1), std::max<int64_t>(1, most));
   return dim3((unsigned)g, (unsigned)slabs);
 }
 // rows per block for the row-tiled apply passes: ~16384 blocks for tensors of >= 40M elements,

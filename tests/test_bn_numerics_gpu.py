@@ -114,3 +114,23 @@ def test_nonfinite_batch_does_not_poison_shift():
     assert torch.isfinite(bn.running_mean).all() and torch.isfinite(bn.running_var).all()
     assert torch.isfinite(y.float()).all()
     _check(bn, x.double(), 1, 5.0)
+
+
+@pytest.mark.parametrize("N,C,H", [(8, 128, 24), (8, 64, 31), (2, 256, 60), (3, 1024, 40)])
+def test_sums_of_small_layers_repeat_bit_for_bit(N, C, H):
+    """Below 8192 rows no more than two blocks add into a shard, so the order of the atomics cannot show."""
+    from deep_vision_amd import nn
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x32 = torch.randn(N, C, H, H, device="cuda", generator=g) + 0.5
+    go = _nhwc(torch.randn(N, C, H, H, device="cuda", generator=g))
+    first = None
+    for _ in range(40):
+        m = nn.BatchNorm2d(C).cuda()
+        x = _nhwc(x32).requires_grad_(True)
+        y = m(x)
+        y.backward(go)
+        out = [y.detach(), x.grad, m.weight.grad, m.bias.grad, m.running_mean, m.running_var]
+        if first is None:
+            first = [t.clone() for t in out]
+        assert all(torch.equal(a, b) for a, b in zip(out, first))
