@@ -20,32 +20,32 @@ BLOCK = 256  # values that share a scale of the 8-bit moments; a block holds val
 def listed():
     return [
         # one pooled feature vector of a served image, forward only: launch latency counts
-        dict(name="layer norm 1 row of 2048", op="layer_norm", rows=1, width=2048, pad=0, dtype="bf16", train=False),
+        dict(name="layer norm, 1 row of 2048", op="layer_norm", rows=1, width=2048, pad=0, dtype="bf16", train=False),
         # odd sizes: rows that are a slice of a wider fp32 buffer
-        dict(name="layer norm 777 x 1001 fp32", op="layer_norm", rows=777, width=1001, pad=7, dtype="fp32", train=True),
+        dict(name="layer norm, 777 x 1001 fp32", op="layer_norm", rows=777, width=1001, pad=7, dtype="fp32", train=True),
         # the last feature map of a batch of 256 images, channels last: 256 x 7 x 7 positions
-        dict(name="layer norm 12544 x 2048", op="layer_norm", rows=12544, width=2048, pad=0, dtype="bf16", train=True),
+        dict(name="layer norm, 12544 x 2048", op="layer_norm", rows=12544, width=2048, pad=0, dtype="bf16", train=True),
         # a first-stage feature map of a batch of 128 images: 128 x 56 x 56 positions, narrow rows
-        dict(name="layer norm 401408 x 256", op="layer_norm", rows=401408, width=256, pad=0, dtype="bf16", train=True),
+        dict(name="layer norm, 401408 x 256", op="layer_norm", rows=401408, width=256, pad=0, dtype="bf16", train=True),
         # validation of a few images against 1000 classes: a loss for each image, no gradient
-        dict(name="cross entropy 8 x 1000 eval", op="xent", rows=8, width=2048, classes=1000, smoothing=0.0,
+        dict(name="cross entropy, 8 x 1000 eval", op="xent", rows=8, width=2048, classes=1000, smoothing=0.0,
              ignored=0.0, bias=True, reduction="none", train=False),
         # the usual training step of a 1000-class classifier
-        dict(name="cross entropy 256 x 1000", op="xent", rows=256, width=2048, classes=1000, smoothing=0.0,
+        dict(name="cross entropy, 256 x 1000", op="xent", rows=256, width=2048, classes=1000, smoothing=0.0,
              ignored=0.0, bias=True, reduction="mean", train=True),
         # odd sizes, smoothed labels, a padded batch whose last rows carry no label
-        dict(name="cross entropy 771 x 20011", op="xent", rows=771, width=1021, classes=20011, smoothing=0.1,
+        dict(name="cross entropy, 771 x 20011", op="xent", rows=771, width=1021, classes=20011, smoothing=0.1,
              ignored=0.2, bias=True, reduction="mean", train=True),
         # many positions against a large label set: the logits would take 2 GiB in 32 bits
-        dict(name="cross entropy 8192 x 65536", op="xent", rows=8192, width=2048, classes=65536, smoothing=0.0,
+        dict(name="cross entropy, 8192 x 65536", op="xent", rows=8192, width=2048, classes=65536, smoothing=0.0,
              ignored=0.1, bias=False, reduction="mean", train=True),
         # LeNet-5: a step that is all latency
-        dict(name="adamw 32 61706 values", op="adamw", tensors=10, values=61706, bits=32),
+        dict(name="adamw 32, 61706 values", op="adamw", tensors=10, values=61706, bits=32),
         # ResNet-50: 161 tensors
-        dict(name="adamw 32 25557032 values", op="adamw", tensors=161, values=25557032, bits=32),
-        dict(name="adamw 8 25557032 values", op="adamw", tensors=161, values=25557032, bits=8),
+        dict(name="adamw 32, 25557032 values", op="adamw", tensors=161, values=25557032, bits=32),
+        dict(name="adamw 8, 25557032 values", op="adamw", tensors=161, values=25557032, bits=8),
         # VGG-16
-        dict(name="adamw 8 138357544 values", op="adamw", tensors=32, values=138357544, bits=8),
+        dict(name="adamw 8, 138357544 values", op="adamw", tensors=32, values=138357544, bits=8),
     ]
 
 
