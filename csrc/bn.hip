@@ -102,11 +102,16 @@ DV_DEVICE float act_bwd(float dout, float out, int act, float slope) {
 // iteration. Wide layers (C = 1024 / 2048 at 14x14 / 7x7) have few rows: slabs keep >= ~4
 // blocks per CU in flight there instead of a few hundred row blocks.
 constexpr int SLAB_TPR = 64;
+// threads across a slab: SLAB_TPR, or half of that where the row's `cg` vectors are cut into more slabs
+DV_DEVICE int slab_tpr(int cg, int slabs) {
+  const int t = (cg + SLAB_TPR - 1) / SLAB_TPR < slabs ? SLAB_TPR / 2 : SLAB_TPR;
+  return cg < t ? cg : t;
+}
 struct SlabTile {
   int cg, tpr, rpi, lane_c, lane_r, g;
   int64_t r0, r1;
   DV_DEVICE SlabTile(int C, int VEC, int64_t rows) {
-    cg = C / VEC; tpr = cg < SLAB_TPR ? cg : SLAB_TPR; rpi = NT / tpr;
+    cg = C / VEC; tpr = slab_tpr(cg, gridDim.y); rpi = NT / tpr;
     lane_c = threadIdx.x % tpr; lane_r = threadIdx.x / tpr;
     g = blockIdx.y * tpr + lane_c;
     const int64_t rpb = (rows + gridDim.x - 1) / gridDim.x;
@@ -547,13 +552,19 @@ int g_reduce_blocks = 1024;  // benchmarking override (dv_bn_tuning)
 int g_reduce_unroll = 2;
 // (row blocks, channel slabs): ~4 blocks per CU (8 with several slabs), >= 32 rows per block. Below 8192 rows
 // at most two blocks a shard: their order then does not matter (0 + a + b == 0 + b + a), so small layers'
-// sums repeat bit for bit; a third adder turned single bf16 values of dx over from run to run.
+// sums repeat bit for bit; a third adder turned single bf16 values of dx over from run to run. The blocks this
+// takes away come back as slabs of 32 vectors: forward and backward of 6272 x 512 28.5 us (28.9 without the
+// limit, 32.7 with it and slabs of 64), 8183 x 1024 43.7 (45.4, 50.2). Rows of 256 channels and fewer gain nothing
+// from slabs of 16 and pay for the repeatability: 8183 x 256 24.1 us (22.5).
 inline dim3 reduce_grid(int64_t rows, int C) {
-  const int v = vec_for(C), cg = C / v, tpr = cg < SLAB_TPR ? cg : SLAB_TPR;
-  const int slabs = (cg + tpr - 1) / tpr;
-  const int64_t target = (int64_t)g_reduce_blocks * (slabs > 1 ? 2 : 1) / slabs;
-  const int64_t most = rows < 8192 ? std::min<int64_t>(rows / 32, 2 * SHARDS) : rows / 32;
-  const int64_t g = std::min<int64_t>(std::max<int64_t>(target, 1), std::max<int64_t>(1, most));
+  const int v = vec_for(C), cg = C / v;
+  int slabs = (cg + SLAB_TPR - 1) / SLAB_TPR;
+  const int64_t target = std::max<int64_t>((int64_t)g_reduce_blocks * (slabs > 1 ? 2 : 1) / slabs, 1);
+  int64_t g = std::min<int64_t>(target, std::max<int64_t>(1, rows / 32));
+  if (rows < 8192 && g > 2 * SHARDS) {
+    g = 2 * SHARDS;
+    if (cg > SLAB_TPR / 2) slabs = (cg + SLAB_TPR / 2 - 1) / (SLAB_TPR / 2);
+  }
   return dim3((unsigned)g, (unsigned)slabs);
 }
 // rows per block for the row-tiled apply passes: ~16384 blocks for tensors of >= 40M elements,

@@ -134,3 +134,32 @@ def test_sums_of_small_layers_repeat_bit_for_bit(N, C, H):
         if first is None:
             first = [t.clone() for t in out]
         assert all(torch.equal(a, b) for a, b in zip(out, first))
+
+
+@pytest.mark.parametrize("N,C,H", [(128, 512, 7), (167, 1024, 7), (40, 264, 14), (32, 520, 14), (64, 2048, 8), (85, 320, 7)])
+def test_narrow_slabs_repeat_and_cover_every_channel(N, C, H):
+    """4128 to 8191 rows: the channels are cut into slabs of 256, the last one in part. A channel's sums are
+    those of up to 8191 bf16 products in fp32, each block's some 64 in a row: within 128 * 2^-24 of the sum of sizes."""
+    from deep_vision_amd import nn
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x32 = torch.randn(N, C, H, H, device="cuda", generator=g) + 0.5
+    go = _nhwc(torch.randn(N, C, H, H, device="cuda", generator=g))
+    first = None
+    for _ in range(10):
+        m = nn.BatchNorm2d(C, momentum=1.0).cuda()
+        x = _nhwc(x32).requires_grad_(True)
+        y = m(x)
+        y.backward(go)
+        out = [y.detach(), x.grad, m.weight.grad, m.bias.grad, m.running_mean, m.running_var]
+        if first is None:
+            first = [t.clone() for t in out]
+        assert all(torch.equal(a, b) for a, b in zip(out, first))
+    _check(m, _nhwc(x32).double(), 0, 0.5)
+    want, size = go.double().sum((0, 2, 3)), go.double().abs().sum((0, 2, 3))
+    assert ((m.bias.grad.double() - want).abs() <= 128 * 2.0 ** -24 * size).all()
+    xd = _nhwc(x32).double()
+    xh = (xd - xd.mean((0, 2, 3), keepdim=True)) / (xd.var((0, 2, 3), unbiased=False, keepdim=True) + m.eps).sqrt()
+    want, size = (go.double() * xh).sum((0, 2, 3)), (go.double() * xh).abs().sum((0, 2, 3))
+    # the mean and the deviation carry a few more roundings of the sums they come from
+    assert ((m.weight.grad.double() - want).abs() <= 256 * 2.0 ** -24 * size + 1e-6 * go.double().abs().sum((0, 2, 3))).all()
