@@ -246,6 +246,24 @@ def track_leaves(ctx, *leaves):
             del _GRAPHS[k]
 
 
+def updates_seen(t):
+    """What ``refuse_updated`` needs of a tensor that a backward pass is going to read again: the update count
+    of the parameter it is, or is a view of (train.optim counts), or None."""
+    if t is None:
+        return None
+    count = getattr(t if t._base is None else t._base, "_dv_updates", None)
+    return None if count is None else (count, count[0], t.data_ptr())
+
+
+def refuse_updated(what, name, t, seen):
+    """Raise where an optimizer has moved ``t`` since ``updates_seen(t)``. The fused optimizers write through raw
+    pointers, which autograd's own check of saved tensors cannot notice. (A tensor that saved-tensor hooks
+    brought back from elsewhere still holds what the forward pass saw.)"""
+    if seen is not None and seen[0][0] != seen[1] and (t.data_ptr() == seen[2] or getattr(t, "_dv_updates", None) is seen[0]):
+        raise RuntimeError(f"{what}: an optimizer has updated the {name} since the forward pass, whose results the gradients "
+                           "need: call backward() before step()")
+
+
 def same_device(what, x, *others):
     """Every tensor of ``others`` (None allowed) lives where ``x`` does."""
     for t in others:

@@ -8,8 +8,8 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as TF
 
-from .common import (BF16, F32, accumulation_sink, fast_apply, first_derivative_only, lib, native, on_device, ptr, same_device,
-                     stream_handle, track_leaves)
+from .common import (BF16, F32, accumulation_sink, fast_apply, first_derivative_only, lib, native, on_device, ptr, refuse_updated,
+                     same_device, stream_handle, track_leaves, updates_seen)
 
 
 class _XentFn(torch.autograd.Function):
@@ -144,6 +144,8 @@ class _LinearXentFn(torch.autograd.Function):
             track_leaves(ctx, *leaf, weight, bias)
             loss, saved = _linear_xent_forward(x, weight, bias, labels, smoothing, ignore_index, reduction, True)
         ctx.cfg = (smoothing, ignore_index, reduction)
+        # backward reads the parameter's own operand and the bias again, unless the forward pass made copies
+        ctx.seen = (updates_seen(weight if saved[2] is None else None), updates_seen(bias if saved[3] is bias else None))
         ctx.save_for_backward(x, weight, bias, *saved)
         return loss
 
@@ -155,6 +157,8 @@ class _LinearXentFn(torch.autograd.Function):
 def _linear_xent_backward(ctx, go, sinks):
     x, weight, bias, labels, xk, wk, b, stats = ctx.saved_tensors
     smoothing, ignore_index, reduction = ctx.cfg
+    refuse_updated("linear_cross_entropy", "weight", weight, ctx.seen[0])
+    refuse_updated("linear_cross_entropy", "bias", bias, ctx.seen[1])
     N, D = x.shape
     V, Dp = weight.shape[0], (D + 63) // 64 * 64
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
@@ -166,7 +170,7 @@ def _linear_xent_backward(ctx, go, sinks):
     if go.dtype != F32 or not go.is_contiguous():
         go = go.to(F32).contiguous()
     # (the engine runs a node on the device and stream of its forward pass)
-    if wk is None:  # the parameter's operand, as it is now
+    if wk is None:  # the parameter's operand
         wk = _operand(weight, Dp)
     args = _linear_xent_args(xk, wk, b, labels, V, Dp, D, ignore_index, smoothing, reduction)
     ws = x.new_empty(lib().linear_xent_bwd_bytes(*args, int(need_x), int(need_w), int(need_b)), dtype=torch.uint8)

@@ -12,8 +12,8 @@ import math
 import torch
 import torch.nn.functional as TF
 
-from .common import (BF16, F32, accumulation_sink, fast_apply, first_derivative_only, lib, native, on_device, ptr, same_device,
-                     stream_handle, track_leaves)
+from .common import (BF16, F32, accumulation_sink, fast_apply, first_derivative_only, lib, native, on_device, ptr, refuse_updated,
+                     same_device, stream_handle, track_leaves, updates_seen)
 
 
 def _rows(t, D):
@@ -50,6 +50,7 @@ class _LayerNormFn(torch.autograd.Function):
             track_leaves(ctx, *leaves)
             x2, ld = _rows(x, x.shape[-1])
             y, stats = _forward(x2, ld, _dense(weight), _dense(bias), eps, True)
+        ctx.seen = updates_seen(weight)
         ctx.save_for_backward(x, weight, bias, stats)
         return y if x.dim() == 2 else y.view(x.shape)
 
@@ -61,6 +62,7 @@ class _LayerNormFn(torch.autograd.Function):
 def _backward(ctx, dy, sinks):
     # runs on autograd's device thread, where every Python step costs more than in the forward pass
     x, weight, bias, stats = ctx.saved_tensors
+    refuse_updated("layer_norm", "weight", weight, ctx.seen)
     need_x, need_w, need_b = ctx.needs_input_grad[:3]
     dtype = x.dtype
     dx = (torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=dtype, device=x.device)) if need_x else None

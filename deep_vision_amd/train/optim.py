@@ -103,6 +103,10 @@ class _FlatOptimizer(torch.optim.Optimizer):
                 p._dv_off = off
         f = dict(param=pflat, grad=gflat, views=views, gviews=gviews, offsets=offs, step=0, first=True, shared=shared)
         f["ptrs"] = [v.data_ptr() for v in views]
+        for p in ps:
+            if not hasattr(p, "_dv_updates"):
+                p._dv_updates = [0]
+        f["updates"] = [p._dv_updates for p in ps]
         f["states"] = self._new_states(f)
         if old is not None:  # re-bound after the parameters moved: carry the optimizer state over
             f["step"], f["first"] = old["step"], old["first"]
@@ -186,7 +190,20 @@ class _FlatOptimizer(torch.optim.Optimizer):
                 continue
             f["step"] += 1
             f["first"] = False
+            self._count_updates(f, [(0, f["param"].numel())])
             self._write_hp(group, f)
+
+    @staticmethod
+    def _count_updates(f, segs):
+        """Count the update of each parameter in the segments ``segs``: the kernels write through raw pointers, so a
+        backward pass that reads a parameter again cannot tell from its version (ops.common.refuse_updated)."""
+        if len(segs) == 1 and segs[0][1] == f["param"].numel():
+            for count in f["updates"]:
+                count[0] += 1
+            return
+        for count, (at, n) in zip(f["updates"], f["offsets"]):
+            if any(off <= at and at + n <= off + k for off, k in segs):
+                count[0] += 1
 
     def _hp_ptr(self, f):
         hp = f.get("hp")
@@ -311,6 +328,7 @@ class _FlatOptimizer(torch.optim.Optimizer):
                 self._write_hp(group, f)
             for off, n in segs:
                 self._update(group, f, off, n, grad_scale)
+            self._count_updates(f, segs)
             f["first"] = False
         if guard:
             lib().nonfinite_tally(ptr(self._dguard), stream_handle())  # counters; re-arms the flag
