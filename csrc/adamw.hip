@@ -21,7 +21,9 @@
 //  * One multiplication by 2^-120 puts e4m3's exponent field and fraction where the float's are
 //    (its values under the least normal one become the float's denormals), so the code is the
 //    rounded bit pattern shifted down by 20, and decoding is the reverse.
-//  * A value that is not finite becomes the NaN code, and makes the step's parameter NaN as well.
+//  * A value that is not finite becomes the NaN code and is read back as NaN: its parameter is NaN from the next
+//    step on at the latest, as with 32-bit moments it stays NaN or stuck. The scale is that of the block's finite
+//    values, which keep theirs.
 #include "common.h"
 #include "kernels.h"
 
@@ -112,6 +114,9 @@ DV_DEVICE uint32_t mix(uint32_t h) {
   h *= 0x5D2A4B35u;
   return h ^ (h >> 16);
 }
+// whether one of the four codes is NaN
+DV_DEVICE bool any_nan(uint32_t codes) { return ((codes & 0x7f7f7f7f) + 0x01010101) & 0x80808080; }
+// of any code but NaN
 DV_DEVICE float from8(uint32_t code, float scale) {
   return __uint_as_float((code & 0x7f) << 20 | (code & 0x80) << 24) * 0x1p+120f * scale;
 }
@@ -121,6 +126,16 @@ DV_DEVICE uint32_t to8(float t, float up, uint32_t bits) {
   if (!(s < 1e30f)) return 0x7f;
   const uint32_t code = (__float_as_uint(s * 0x1p-120f) + bits) >> 20;
   return code < 126 ? code : 126;
+}
+
+// the wave's largest |t|, infinities apart; `top`: this lane's
+DV_DEVICE float finite_max(float top, const float (&t)[4]) {
+  top = wave_max(top);
+  if (top < INFINITY) return top;
+  top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) top = fabsf(t[e]) < INFINITY ? fmaxf(top, fabsf(t[e])) : top;
+  return wave_max(top);
 }
 
 __global__ __launch_bounds__(NT) void adamw8_kernel(DvAdamW a, const DvAdamWChunk* __restrict__ chunks, float* __restrict__ p,
@@ -154,10 +169,20 @@ __global__ __launch_bounds__(NT) void adamw8_kernel(DvAdamW a, const DvAdamWChun
     float mtop = 0.f, rtop = 0.f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-#pragma clang fp contract(off)
       mv[e] = from8(mq >> (8 * e), msc);
-      const float r = from8(rq >> (8 * e), rsc);
-      float v = r * r;
+      rv[e] = from8(rq >> (8 * e), rsc);
+    }
+    if (__any(any_nan(mq) || any_nan(rq))) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if ((mq >> (8 * e) & 0x7f) == 0x7f) mv[e] = NAN;
+        if ((rq >> (8 * e) & 0x7f) == 0x7f) rv[e] = NAN;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+#pragma clang fp contract(off)
+      float v = rv[e] * rv[e];
       moments(c, gv[e] * c.gscale, mv[e], v);
       rv[e] = sqrtf(v);
       if (e >= left) mv[e] = rv[e] = 0.f;  // behind the tensor's end the state stays zero
@@ -165,8 +190,8 @@ __global__ __launch_bounds__(NT) void adamw8_kernel(DvAdamW a, const DvAdamWChun
       rtop = fmaxf(rtop, rv[e]);
       pv[e] = update(c, pv[e], mv[e], rv[e]);
     }
-    mtop = wave_max(mtop);
-    rtop = wave_max(rtop);
+    mtop = finite_max(mtop, mv);  // (fmaxf has left NaN out)
+    rtop = finite_max(rtop, rv);
     const float mup = mtop >= 0x1p-100f ? 448.f / mtop : 0.f, rup = rtop >= 0x1p-100f ? 448.f / rtop : 0.f;
     uint32_t mc = 0, rc = 0;
 #pragma unroll

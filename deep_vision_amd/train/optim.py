@@ -562,9 +562,10 @@ class FusedAdamW(_FlatOptimizer):
         """Blocks ``t`` [blocks][256] as codes and scales, the kernel's arithmetic (csrc/adamw.hip)."""
         if not t.numel():
             return
-        top = t.abs().amax(1, keepdim=True)
+        size = t.abs()
+        top = torch.where(size < math.inf, size, 0.0).amax(1, keepdim=True)  # of what is finite
         up = torch.where(top >= 2.0 ** -100, torch.full_like(top, 448.0) / top, torch.zeros_like(top))
-        s = t.abs() * up
+        s = size * up
         code = (((s * 2.0 ** -120).view(torch.int32).long() + noise) >> 20).clamp_(max=126)
         code = torch.where(s < 1e30, code, 127)
         if name == "exp_avg":

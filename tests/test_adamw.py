@@ -370,3 +370,60 @@ def test_past_32_bits_of_values(bits):
     for k in a:
         if k.endswith("_scale") or bits == 32:
             torch.testing.assert_close(a[k], b[k], rtol=0.3 if bits == 8 else 0, atol=0)
+
+
+def poisoned(dev, bad, always=False, steps=3):
+    """(parameters, states) of 8-bit runs whose first step's gradient (``always``: every step's) holds
+    ``bad`` {(tensor, place): value}, step by step."""
+    params, opt = make(dev, 8, sizes=[600, 300, 256])
+    out = []
+    for step in range(steps):
+        grads = tensors([600, 300, 256], "cpu", 100 + step)
+        if always or step == 0:
+            for (i, at), v in bad.items():
+                grads[i][at] = v
+        for p, g in zip(params, grads):
+            p.grad.copy_(g)
+        opt.step()
+        out.append(([p.detach().cpu().clone() for p in params], {k: t.cpu().clone() for k, t in states(opt).items()}))
+    return out
+
+
+INF, NAN = float("inf"), float("nan")
+BAD = [{(0, 300): NAN}, {(0, 300): INF}, {(0, 5): -INF, (0, 300): 1e25}, {(0, 599): INF, (2, 0): NAN},
+       {(1, k): NAN for k in range(300)}, {(1, k): INF for k in range(256)}]
+
+
+@pytest.mark.parametrize("bad", BAD)
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(DEV, marks=gpu)])
+def test_a_value_that_is_not_finite_stays_alone(dev, bad):
+    """The others of its block go on as beside a zero; itself is NaN from the second step on. (A finite gradient
+    whose square overflows leaves the first step's parameter finite, and its first moment sets its block's scale.)"""
+    runs = poisoned(dev, bad), poisoned(dev, {k: 0.0 for k in bad}, always=True)
+    starts = (0, 768, 1280)
+    places = torch.tensor([starts[i] + at for i, at in bad])
+    apart = torch.zeros(1536, dtype=torch.bool)  # places that are not those of the clean run
+    apart[places] = True
+    block = {starts[i] // 256 + at // 256 for (i, at), v in bad.items() if abs(v) < INF}
+    for b in block:
+        apart[b * 256:b * 256 + 256] = True
+    for step, ((p, s), (cp, cs)) in enumerate(zip(*runs)):
+        for name in ("exp_avg", "exp_avg_root"):
+            scale, clean = s[name + "_scale"], cs[name + "_scale"]
+            assert scale.isfinite().all()
+            assert all(scale[b] == clean[b] for b in range(6) if b not in block)
+            assert torch.equal(s[name][~apart], cs[name][~apart])
+            codes = s[name].view(torch.float8_e4m3fn).float()
+            assert codes.isfinite().sum() == 1536 - len(bad) + (len(block) if name == "exp_avg" else 0)
+        for i, (a, b) in enumerate(zip(p, cp)):
+            keep = ~apart[starts[i]:starts[i] + a.numel()]
+            assert torch.equal(a[keep], b[keep])
+            assert a.isnan().sum() == sum(j == i and (step > 0 or not abs(v) < INF) for (j, _), v in bad.items())
+
+
+@gpu
+@pytest.mark.parametrize("bad", BAD)
+def test_host_and_kernel_agree_behind_a_value_that_is_not_finite(bad):
+    for (gp, gs), (cp, cs) in zip(poisoned(DEV, bad), poisoned("cpu", bad)):
+        assert all(torch.equal(gs[k], cs[k]) for k in cs)
+        assert all(torch.equal(a.isnan(), b.isnan()) for a, b in zip(gp, cp))
