@@ -427,3 +427,23 @@ def test_host_and_kernel_agree_behind_a_value_that_is_not_finite(bad):
     for (gp, gs), (cp, cs) in zip(poisoned(DEV, bad), poisoned("cpu", bad)):
         assert all(torch.equal(gs[k], cs[k]) for k in cs)
         assert all(torch.equal(a.isnan(), b.isnan()) for a, b in zip(gp, cp))
+
+
+@pytest.mark.parametrize("b2", [0.99, 0.997])
+def test_8_bit_second_moment_settles_above_its_mean(b2):
+    """What the documentation says of v. A step moves the root by at most (1 - b2) / 2 E|g^2 / v - 1| r = 0.49
+    (1 - b2) r in the mean, and the block's scale by as much: rounding adds at most their product with a code's step,
+    r / 8, to the root's square each step, which the decay forgets by 1 - b2: at most 2 * 0.49 / 8 = 12 % in balance."""
+    n, steps = 8192, int(6 / (1 - b2))
+    g = torch.Generator().manual_seed(0)
+    v = torch.zeros(n)
+    p = torch.nn.Parameter(torch.zeros(n))
+    opt = FusedAdamW([p], lr=0.0, betas=(0.9, b2), state_bits=8)
+    for _ in range(steps):
+        p.grad.copy_(torch.randn(n, generator=g))
+        v = b2 * v + (1 - b2) * p.grad ** 2
+        opt.step()
+    s = opt.flat_states()[0]
+    r = s["exp_avg_root"].float().view(-1, 256) * s["exp_avg_root_scale"][:, None]
+    assert 0.01 < (r ** 2).mean() / v.mean() - 1 < 0.13
+    assert -0.01 < r.mean() / v.sqrt().mean() - 1 < 0.07  # the mean of roots moves by no more than half of that
