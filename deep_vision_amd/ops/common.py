@@ -13,6 +13,7 @@ import os
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 
 from .._ext import current_device, lib, ptr, stream_handle  # noqa: F401
 
@@ -220,6 +221,13 @@ def first_derivative_only(what, backward, ctx, go):
     with torch.no_grad():
         grads = backward(ctx, go, False)
     return tuple(g if g is None or not inputs else _NoSecondDerivative.apply(what, g, *inputs) for g in grads)
+
+
+def observed():
+    """Whether forward-mode differentiation or a trace is watching. Both see autograd functions and torch
+    operations only: a kernel launched outside of one would leave a dual number without its tangent (a derivative
+    of zero) and the trace with an uninitialised result. Inside of one the first raises and the second records it."""
+    return forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None
 
 
 _GRAPHS = {}  # id(leaf) -> [(weak references to an autograd node that uses it and to the leaf, the node's stream)]

@@ -8,8 +8,8 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as TF
 
-from .common import (BF16, F32, accumulation_sink, fast_apply, first_derivative_only, lib, native, on_device, ptr, refuse_updated,
-                     same_device, stream_handle, track_leaves, updates_seen)
+from .common import (BF16, F32, accumulation_sink, fast_apply, first_derivative_only, lib, native, observed, on_device, ptr,
+                     refuse_updated, same_device, stream_handle, track_leaves, updates_seen)
 
 
 class _XentFn(torch.autograd.Function):
@@ -230,7 +230,7 @@ def linear_cross_entropy(x, weight, labels, bias=None, label_smoothing=0.0, igno
     if x2.dtype != BF16:
         x2 = x2.to(BF16)
     args = (x2, weight, bias, flat if flat.is_contiguous() else flat.contiguous(), float(label_smoothing), int(ignore_index), code)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, weight, bias)):
+    if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x2, weight, bias))) or observed():
         loss = _apply_linear_xent(*args, (x,))
     else:
         with on_device(x):

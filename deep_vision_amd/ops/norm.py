@@ -12,8 +12,8 @@ import math
 import torch
 import torch.nn.functional as TF
 
-from .common import (BF16, F32, accumulation_sink, fast_apply, first_derivative_only, lib, native, on_device, ptr, refuse_updated,
-                     same_device, stream_handle, track_leaves, updates_seen)
+from .common import (BF16, F32, accumulation_sink, fast_apply, first_derivative_only, lib, native, observed, on_device, ptr,
+                     refuse_updated, same_device, stream_handle, track_leaves, updates_seen)
 
 
 def _rows(t, D):
@@ -99,7 +99,7 @@ def layer_norm(x, normalized_shape, weight=None, bias=None, eps=1e-5):
     if not 0 < eps < math.inf:
         raise ValueError(f"layer_norm: eps must be positive and finite, got {eps}")
     on_gpu = native(x)
-    train = torch.is_grad_enabled() and x.requires_grad
+    train = (torch.is_grad_enabled() and x.requires_grad) or observed()
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue

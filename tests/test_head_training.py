@@ -114,3 +114,56 @@ def test_a_step_between_the_passes_is_refused_on_the_gpu(op):
     if op == "layer_norm":  # what was saved elsewhere is what the forward pass saw
         assert torch.equal(torch.autograd.grad(kept.sum(), x)[0], want)
     call(op, norm_layer, fc, x, y).sum().backward()
+
+
+# ---------------------------------------------------------------- what watches a call beside autograd
+def tensors_of(op):
+    x = torch.randn(4, 8)
+    if op == "layer_norm":
+        return [x, torch.ones(8), torch.zeros(8)], lambda x, w, b: F.layer_norm(x, 8, w, b)
+    y = torch.zeros(4, dtype=torch.int64)
+    return [x, torch.randn(5, 8).bfloat16(), torch.zeros(5)], lambda x, w, b: F.linear_cross_entropy(x, w, y, b)
+
+
+@pytest.mark.parametrize("op", ["layer_norm", "linear_cross_entropy"])
+@pytest.mark.parametrize("no_grad", [False, True])
+def test_forward_mode_is_refused(on_cpu, op, no_grad):
+    from torch.autograd import forward_ad
+
+    args, f = tensors_of(op)
+    for i in range(3):
+        with forward_ad.dual_level(), torch.set_grad_enabled(not no_grad):
+            dual = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(args)]
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                f(*dual)
+    assert not f(*args).requires_grad
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("op", ["layer_norm", "linear_cross_entropy"])
+@pytest.mark.parametrize("no_grad", [False, True])
+def test_a_trace_records_the_operator(on_cpu, op, no_grad):
+    args, f = tensors_of(op)
+    with torch.set_grad_enabled(not no_grad):
+        traced = torch.jit.trace(lambda x, w, b: f(x, w, b), args, check_trace=False)
+    nodes = [n.kind() for n in traced.graph.nodes()]
+    assert "prim::PythonOp" in nodes and "aten::empty" not in nodes
+    before = len(on_cpu["kernels"].calls)
+    traced(*args)
+    assert len(on_cpu["kernels"].calls) > before
+
+
+@gpu
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("op", ["layer_norm", "linear_cross_entropy"])
+def test_a_traced_call_gives_the_operators_results(op):
+    args, f = tensors_of(op)
+    args = [t.to(DEV) for t in args]
+    if op == "linear_cross_entropy":
+        y = torch.tensor([0, 4, 2, 1], device=DEV)
+        f = lambda x, w, b: F.linear_cross_entropy(x, w, y, b)  # noqa: E731
+    traced = torch.jit.trace(f, args, check_trace=False)
+    for k in range(3):
+        now = [t + k if t.dtype == torch.float32 else t for t in args]
+        torch.empty(1 << 20, device=DEV).fill_(float("nan"))
+        assert torch.equal(traced(*now), f(*now))
