@@ -35,6 +35,14 @@ from typing import Callable, Sequence
 import torch
 
 
+def _detached(outputs):
+    """A step's outputs without their autograd graphs, which backward has used up: kept alive, their nodes would
+    hold on to the stream they were built on and to what they saved."""
+    from torch.utils._pytree import tree_map
+
+    return tree_map(lambda t: t.detach() if isinstance(t, torch.Tensor) else t, outputs)
+
+
 class CapturedStep:
     """``step_fn(*static_inputs)`` (zero_grad, forward, loss, backward, optimizer.step) captured once
     after ``warmup`` eager iterations on a side stream, then replayed by ``__call__``.
@@ -78,7 +86,7 @@ class CapturedStep:
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s), capture_warmup():
             for _ in range(max(1, warmup)):  # real steps: allocator warm-up, first-step optimizer state
-                self.warmup_outputs = self.step_fn(*self.static_inputs)
+                self.warmup_outputs = _detached(self.step_fn(*self.static_inputs))
         torch.cuda.current_stream().wait_stream(s)
         from ..ops.act import step_counter
 
@@ -93,7 +101,7 @@ class CapturedStep:
         from ..parallel.watchdog import suspend_polling
 
         with suspend_polling(), torch.cuda.graph(self.graph, stream=s):  # no event queries mid-capture
-            self.outputs = self.step_fn(*self.static_inputs)
+            self.outputs = _detached(self.step_fn(*self.static_inputs))
         # the capture executed nothing: undo its host-side bookkeeping
         for f, h in zip(self.opt._flat, host):
             if f is not None:

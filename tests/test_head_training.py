@@ -167,3 +167,93 @@ def test_a_traced_call_gives_the_operators_results(op):
         now = [t + k if t.dtype == torch.float32 else t for t in args]
         torch.empty(1 << 20, device=DEV).fill_(float("nan"))
         assert torch.equal(traced(*now), f(*now))
+
+
+# ---------------------------------------------------------------- several captured signatures
+class Fake:
+    """Stands in for a stream or a graph."""
+
+    handles = 100
+
+    def __init__(self, *args, **kw):
+        Fake.handles += 1
+        self.handle = Fake.handles
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+def test_every_signature_is_captured_beside_the_outputs_of_the_others(on_cpu, monkeypatch):
+    """Each capture has a stream of its own; a step that returns its loss as it is leaves no graph behind."""
+    import contextlib
+
+    from deep_vision_amd.ops import act
+    from deep_vision_amd.train.graph import CapturedStep
+
+    @contextlib.contextmanager
+    def within(stream, capturing=False):
+        old = dict(on_cpu)
+        on_cpu.update(stream=stream.handle, capturing=capturing)
+        yield
+        on_cpu.update(old)
+
+    for name, to in (("Stream", Fake), ("CUDAGraph", Fake), ("current_stream", Fake), ("synchronize", lambda: None),
+                     ("current_device", lambda: 0), ("stream", within),
+                     ("graph", lambda g, stream: within(stream, True))):
+        monkeypatch.setattr(torch.cuda, name, to)
+    monkeypatch.setattr(act, "step_counter", lambda dev: None)
+    norm_layer, fc = head()
+    opt = FusedSGD([*norm_layer.parameters(), *fc.parameters()], lr=0.1)
+
+    def step(x, y):
+        opt.zero_grad()
+        loss = call("linear_cross_entropy", None, fc, norm_layer(x), y).sum()
+        loss.backward()
+        opt.step()
+        return loss, {"again": [loss, 3]}
+
+    kept = []
+    for rows in (4, 3, 2):
+        kept.append(CapturedStep(step, opt, (torch.randn(rows, 8).bfloat16(), torch.zeros(rows, dtype=torch.int64)), warmup=1))
+    for cap in kept:
+        assert cap.outputs[0].grad_fn is None and cap.warmup_outputs[1]["again"][0].grad_fn is None
+        assert cap.outputs[1]["again"][1] == 3
+
+
+@gpu
+def test_two_batch_sizes_through_the_trainers_captured_step():
+    """Replays of either signature, in turn, against eager steps: losses and parameters as in eager training, but
+    for the bias corrections (in 32 bits on the device, 64 on the host)."""
+    from deep_vision_amd.train.graph import GraphedTrainStep
+
+    def make():
+        norm_layer, fc = head(128, 300, DEV)
+        model = torch.nn.Sequential(norm_layer, fc)
+        opt = FusedAdamW(model.parameters(), lr=1e-3)
+
+        def forward_loss(x, y):
+            z = norm_layer(x)
+            return F.linear_cross_entropy(z, fc.weight, y, fc.bias), z
+
+        def eager(x, y):
+            opt.zero_grad()
+            loss, z = forward_loss(x, y)
+            loss.backward()
+            opt.step()
+            return loss.detach(), z.detach()
+
+        return model, opt, forward_loss, eager
+
+    model, opt, forward_loss, eager = make()
+    graphed = GraphedTrainStep(model, opt, forward_loss, eager)
+    twin, _, _, plain = make()
+    g = torch.Generator(device=DEV).manual_seed(0)
+    for k, rows in enumerate((64, 64, 24, 64, 24, 24, 64)):
+        x = torch.randn(rows, 128, generator=g, device=DEV).bfloat16()
+        y = torch.randint(0, 300, (rows,), generator=g, device=DEV)
+        a, b = graphed(x, y), plain(x, y)
+        torch.cuda.synchronize()
+        torch.testing.assert_close(a[0], b[0], rtol=2e-3, atol=2e-3)
+        for p, q in zip(model.parameters(), twin.parameters()):
+            assert (p - q).norm() <= 1e-3 * q.norm(), k
+    assert len(graphed.graphs) == 2
