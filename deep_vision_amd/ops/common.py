@@ -10,6 +10,7 @@ GPU tensor conventions (all native ops):
 from __future__ import annotations
 
 import os
+import threading
 import weakref
 
 import torch
@@ -192,7 +193,7 @@ def accumulation_sink(ctx, index, param):
     if sink is None or param._backward_hooks:
         return None
     stream = stream_handle()
-    if any(e[2] != stream and e[0]() is not None and e[1]() is param for e in _GRAPHS.get(id(param), ())):
+    if any(e[2] != stream and _alive(e, param) for e in _GRAPHS.get(id(param), ())):
         return None
     try:
         return sink if torch._C._will_engine_execute_node(ctx.next_functions[index][0]) else None
@@ -230,28 +231,39 @@ def observed():
     return forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None
 
 
-_GRAPHS = {}  # id(leaf) -> [(weak references to an autograd node that uses it and to the leaf, the node's stream)]
+# id(leaf) -> [(weak references to an autograd node that uses it and to the leaf, the node's stream)]; lists are
+# replaced, never changed, so that a reader needs no lock
+_GRAPHS = {}
+_GRAPHS_LOCK = threading.Lock()
+_GRAPHS_KEEP = 4096
+_graphs_limit = _GRAPHS_KEEP
+
+
+def _alive(e, leaf):
+    return e[0]() is not None and e[1]() is leaf
 
 
 def track_leaves(ctx, *leaves):
     """Remember which stream the live graphs of ``leaves`` were built on, and refuse to capture a new
     one while an older lives: the leaf's gradient accumulation belongs to the older graph's stream,
     and a captured backward pass that joins a stream outside the capture ends the process."""
+    global _graphs_limit
     stream = stream_handle()
     capturing = torch.cuda.is_current_stream_capturing()
     me = weakref.ref(ctx)
-    for t in leaves:
-        if t is None or not t.requires_grad or not t.is_leaf:
-            continue
-        alive = [e for e in _GRAPHS.get(id(t), ()) if e[0]() is not None and e[1]() is t]
-        if capturing and any(e[2] != stream for e in alive):
-            raise RuntimeError("an eager autograd graph of this tensor is still alive (a loss or output that holds it): "
-                               "delete it before capturing a backward pass over the same tensor")
-        alive.append((me, weakref.ref(t), stream))
-        _GRAPHS[id(t)] = alive
-    if len(_GRAPHS) > 4096:
-        for k in [k for k, v in _GRAPHS.items() if all(e[0]() is None for e in v)]:
-            del _GRAPHS[k]
+    with _GRAPHS_LOCK:
+        for t in leaves:
+            if t is None or not t.requires_grad or not t.is_leaf:
+                continue
+            alive = [e for e in _GRAPHS.get(id(t), ()) if _alive(e, t)]
+            if capturing and any(e[2] != stream for e in alive):
+                raise RuntimeError("an eager autograd graph of this tensor is still alive (a loss or output that holds it): "
+                                   "delete it before capturing a backward pass over the same tensor")
+            _GRAPHS[id(t)] = [*alive, (me, weakref.ref(t), stream)]
+        if len(_GRAPHS) > _graphs_limit:
+            for k in [k for k, v in _GRAPHS.items() if all(e[0]() is None or e[1]() is None for e in v)]:
+                del _GRAPHS[k]
+            _graphs_limit = max(_GRAPHS_KEEP, 2 * len(_GRAPHS))  # looked over once for as many new leaves again
 
 
 def updates_seen(t):

@@ -257,3 +257,61 @@ def test_two_batch_sizes_through_the_trainers_captured_step():
         for p, q in zip(model.parameters(), twin.parameters()):
             assert (p - q).norm() <= 1e-3 * q.norm(), k
     assert len(graphed.graphs) == 2
+
+
+# ---------------------------------------------------------------- the record of live graphs
+class Track(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *leaves):
+        common.track_leaves(ctx, *leaves)
+        return sum(t.sum() for t in leaves)
+
+    @staticmethod
+    def backward(ctx, g):
+        raise NotImplementedError
+
+
+def test_two_threads_lose_no_live_graph(on_cpu, monkeypatch):
+    import threading
+    import time
+    import weakref
+
+    class Slow:
+        @staticmethod
+        def ref(t):
+            time.sleep(0.05)  # both threads are here at once, unless one waits for the other
+            return weakref.ref(t)
+
+    monkeypatch.setattr(common, "weakref", Slow)
+    for last in range(2):
+        on_cpu.update(stream=1, capturing=False)
+        x = torch.zeros(2, requires_grad=True)
+        out = [None, None]
+
+        def forward(i):
+            out[i] = Track.apply(x)
+
+        threads = [threading.Thread(target=forward, args=(i,)) for i in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        on_cpu.update(stream=2, capturing=True)
+        out[1 - last] = None
+        with pytest.raises(RuntimeError, match="still alive"):
+            Track.apply(x)
+        out[last] = None
+        Track.apply(x)
+
+
+def test_the_record_stays_small_and_is_not_searched_on_every_call(on_cpu, monkeypatch):
+    monkeypatch.setattr(common, "_GRAPHS", {})
+    monkeypatch.setattr(common, "_GRAPHS_KEEP", 8)
+    monkeypatch.setattr(common, "_graphs_limit", 8)
+    for _ in range(100):
+        Track.apply(torch.zeros(1, requires_grad=True))
+    assert len(common._GRAPHS) <= 9
+    leaves = [torch.zeros(1, requires_grad=True) for _ in range(100)]
+    alive = [Track.apply(t) for t in leaves]
+    assert len(common._GRAPHS) >= 100 and common._graphs_limit >= 100
+    del alive
