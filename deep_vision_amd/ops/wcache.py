@@ -58,6 +58,8 @@ def _build_table(device):
             continue
         if e[1].device != device or p.dtype != torch.float32 or not p.is_contiguous():
             continue
+        if e[4] != p.data_ptr():  # moved since its last use: laid out from there by the launch that follows
+            e[2], e[4] = None, p.data_ptr()
         G, pad, mode, Sp = e[5]
         shp = p.shape if p.dim() == 4 else (p.shape[0], p.shape[1], 1, 1)
         O, Ig, R, S = shp
