@@ -8,6 +8,7 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as TF
 
+from . import wcache
 from .common import (BF16, F32, accumulation_sink, fast_apply, first_derivative_only, lib, native, observed, on_device, ptr,
                      refuse_updated, same_device, stream_handle, track_leaves, updates_seen)
 
@@ -97,8 +98,10 @@ def _operands(x, weight, D, Dp):
 
 
 def _cached_weight(weight):
-    """fp32 parameters keep their bf16 operand from step to step (ops/wcache.py)."""
-    return weight.dtype == F32 and isinstance(weight, torch.nn.Parameter) and weight.is_contiguous()
+    """fp32 parameters keep their bf16 operand from step to step (ops/wcache.py). A captured pass that is not
+    part of a captured training step lays out its own, in every replay."""
+    return (weight.dtype == F32 and isinstance(weight, torch.nn.Parameter) and weight.is_contiguous()
+            and not wcache.outdated_in_replays())
 
 
 def _operand(weight, Dp):

@@ -23,6 +23,26 @@ _entries = {}  # key -> [param weakref, buf, epoch, version, data_ptr, geometry]
 _epoch = 0
 _tables = {}  # device -> (n_entries_snapshot, descs, chunks, nchunks)
 ENABLED = True
+_step_captures = 0
+
+
+class step_capture:
+    """Context of the capture of a whole training step (train.graph.CapturedStep): the captured ``after_step()``
+    refreshes the cached operands in every replay."""
+
+    def __enter__(self):
+        global _step_captures
+        _step_captures += 1
+
+    def __exit__(self, *exc):
+        global _step_captures
+        _step_captures -= 1
+
+
+def outdated_in_replays():
+    """Whether the current stream captures something else than a training step. Its replays meet parameters that
+    were changed in between, and this cache has no part in them: a hit records nothing into the graph."""
+    return torch.cuda.is_current_stream_capturing() and not _step_captures
 
 
 def _key(param, G, pad, mode, Sp=0):

@@ -100,7 +100,9 @@ class CapturedStep:
         # and could not allocate it mid-capture
         from ..parallel.watchdog import suspend_polling
 
-        with suspend_polling(), torch.cuda.graph(self.graph, stream=s):  # no event queries mid-capture
+        from ..ops import wcache
+
+        with suspend_polling(), wcache.step_capture(), torch.cuda.graph(self.graph, stream=s):  # no event queries mid-capture
             self.outputs = _detached(self.step_fn(*self.static_inputs))
         # the capture executed nothing: undo its host-side bookkeeping
         for f, h in zip(self.opt._flat, host):

@@ -315,3 +315,53 @@ def test_the_record_stays_small_and_is_not_searched_on_every_call(on_cpu, monkey
     alive = [Track.apply(t) for t in leaves]
     assert len(common._GRAPHS) >= 100 and common._graphs_limit >= 100
     del alive
+
+
+# ---------------------------------------------------------------- the parameter's operand
+@gpu
+@pytest.mark.parametrize("warm", [True, False])
+def test_replays_follow_a_parameter_that_changes(warm):
+    """A graph of the loss and its gradients, no optimizer in it. Parameters change between the replays: by torch
+    operations, by another optimizer, by this package's. Without eager passes before the capture too."""
+    torch.manual_seed(0)
+    fc = dnn.Linear(72, 130).to(DEV)
+    x, y = torch.randn(40, 72, device=DEV).bfloat16().requires_grad_(), torch.randint(0, 130, (40,), device=DEV)
+    leaves = [x, fc.weight, fc.bias]
+
+    def passes(weight=fc.weight):
+        out = F.linear_cross_entropy(x, weight, y, fc.bias)
+        return [out.detach(), *torch.autograd.grad(out, [x, weight, fc.bias])]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    if warm:
+        with torch.cuda.stream(s):
+            passes()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        got = passes()
+        with torch.no_grad():
+            got.append(F.linear_cross_entropy(x, fc.weight, y, fc.bias))
+    eager = passes()  # before any replay
+    assert all(torch.equal(a, b) for a, b in zip(eager, passes(fc.weight.detach().clone().requires_grad_())))
+    fused = FusedSGD(fc.parameters(), lr=0.5)  # the parameters move into its buffer: a new capture below
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        got = passes()
+        with torch.no_grad():
+            got.append(F.linear_cross_entropy(x, fc.weight, y, fc.bias))
+    other = torch.optim.SGD(leaves[1:], lr=0.5)
+    for k in range(6):
+        if k % 3 == 0:
+            with torch.no_grad():
+                fc.weight.add_(0.1 * torch.randn_like(fc.weight))
+        else:
+            for p in leaves[1:]:
+                p.grad.normal_()
+            (other if k % 3 == 1 else fused).step()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = passes(fc.weight.detach().clone().requires_grad_())  # no cached operand
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), k
+        assert torch.equal(got[-1], want[0])
