@@ -346,6 +346,10 @@ def test_replays_follow_a_parameter_that_changes(warm):
     eager = passes()  # before any replay
     assert all(torch.equal(a, b) for a, b in zip(eager, passes(fc.weight.detach().clone().requires_grad_())))
     fused = FusedSGD(fc.parameters(), lr=0.5)  # the parameters move into its buffer: a new capture below
+    if warm:
+        with torch.cuda.stream(s):
+            passes()
+    torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph, stream=s):
         got = passes()
