@@ -19,7 +19,7 @@ import torch
 
 from .._ext import lib, ptr, stream_handle
 
-_entries = {}  # key -> [param weakref, buf, epoch, version, data_ptr, geometry]
+_entries = {}  # key -> [param weakref, buf, epoch, version, data_ptr, geometry, (event, streams behind it) or None]
 _epoch = 0
 _tables = {}  # device -> (n_entries_snapshot, descs, chunks, nchunks)
 ENABLED = True
@@ -58,13 +58,32 @@ def get(param, G, pad, mode, compute, Sp=0):
     e = _entries.get(k)
     if e is not None and e[0]() is param:
         if e[2] == _epoch and e[3] == param._version and e[4] == param.data_ptr():
+            if e[6] is not None:
+                _behind(e[6])
             return e[1]
         buf = compute(e[1])
     else:
         buf = compute(None)
         _tables.pop(buf.device, None)
-    _entries[k] = [weakref.ref(param), buf, _epoch, param._version, param.data_ptr(), (G, pad, mode, Sp)]
+    _entries[k] = [weakref.ref(param), buf, _epoch, param._version, param.data_ptr(), (G, pad, mode, Sp), _laid_out(buf)]
     return buf
+
+
+def _laid_out(buf):
+    """The event behind the launch that fills ``buf``. Streams that only read a parameter need no order among
+    themselves, but the first of them has written its operand."""
+    if not buf.is_cuda or torch.cuda.is_current_stream_capturing():
+        return None
+    event = torch.cuda.Event()
+    event.record()
+    return event, {stream_handle()}
+
+
+def _behind(ready):
+    event, streams = ready
+    if stream_handle() not in streams and not torch.cuda.is_current_stream_capturing():  # (captures begin synchronised)
+        torch.cuda.current_stream().wait_event(event)
+        streams.add(stream_handle())
 
 
 def _build_table(device):
@@ -137,7 +156,8 @@ def after_step(device=None):
     lib().wprep_batched(ptr(t[1]), ptr(t[2]), t[3], stream_handle())
     for k, p in zip(t[4], params):
         e = _entries[k]
-        e[2], e[3], e[4] = _epoch, p._version, p.data_ptr()
+        # (whoever reads the parameters next is ordered behind this step, which has written them too)
+        e[2], e[3], e[4], e[6] = _epoch, p._version, p.data_ptr(), None
 
 
 def clear():

@@ -369,3 +369,26 @@ def test_replays_follow_a_parameter_that_changes(warm):
         want = passes(fc.weight.detach().clone().requires_grad_())  # no cached operand
         assert all(torch.equal(a, b) for a, b in zip(got, want)), k
         assert torch.equal(got[-1], want[0])
+
+
+@gpu
+def test_a_parameter_shared_by_two_streams():
+    """Both streams only read the parameter: the second finds an operand that the first, held up, has yet to lay out."""
+    torch.manual_seed(0)
+    fc = dnn.Linear(256, 1000).to(DEV)
+    x, y = torch.randn(64, 256, device=DEV).bfloat16(), torch.randint(0, 1000, (64,), device=DEV)
+    want = F.linear_cross_entropy(x, fc.weight.detach().clone(), y, fc.bias)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for change in (False, True):
+        if change:
+            with torch.no_grad():
+                fc.weight.mul_(0.5)
+            want = F.linear_cross_entropy(x, fc.weight.detach().clone(), y, fc.bias)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(a), torch.no_grad():
+            torch.cuda._sleep(200_000_000)  # clock ticks: tens of milliseconds, then the stream goes on
+            first = F.linear_cross_entropy(x, fc.weight, y, fc.bias)
+        with torch.cuda.stream(b), torch.no_grad():
+            second = [F.linear_cross_entropy(x, fc.weight, y, fc.bias) for _ in range(2)]
+        torch.cuda.synchronize()
+        assert torch.equal(first, want) and all(torch.equal(t, want) for t in second)

@@ -45,3 +45,41 @@ def test_a_step_refreshes_parameters_that_moved_since_their_last_use(kernels):
     assert kernels.refreshed == 2
     p.data = torch.full((4, 8), 2.0)
     assert layout(p, done) is buf and len(done) == 2
+
+
+def test_other_streams_wait_for_the_layout_once(kernels, monkeypatch):
+    now, waits = {"stream": 1, "capturing": False}, []
+
+    class Event:
+        def record(self):
+            self.stream = now["stream"]
+
+    class Current:
+        def wait_event(self, event):
+            waits.append((now["stream"], event.stream))
+
+    class OnGpu:
+        """A buffer as the cache looks at it."""
+
+        is_cuda, device = True, torch.device("cuda", 0)
+
+    monkeypatch.setattr(wcache, "stream_handle", lambda: now["stream"])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now["capturing"])
+    monkeypatch.setattr(torch.cuda, "Event", Event)
+    monkeypatch.setattr(torch.cuda, "current_stream", Current)
+    p = torch.nn.Parameter(torch.zeros(4, 8))
+
+    def use(stream, capturing=False):
+        now.update(stream=stream, capturing=capturing)
+        wcache.get(p, 1, 8, 0, lambda out: OnGpu())
+
+    for s in (1, 1, 2, 2, 3, 1):
+        use(s)
+    use(4, capturing=True)
+    assert waits == [(2, 1), (3, 1)]
+    with torch.no_grad():
+        p.add_(1)
+    use(2)  # lays it out again
+    for s in (1, 2, 3):
+        use(s)
+    assert waits == [(2, 1), (3, 1), (1, 2), (3, 2)]
