@@ -35,14 +35,6 @@ from typing import Callable, Sequence
 import torch
 
 
-def _detached(outputs):
-    """A step's outputs without their autograd graphs, which backward has used up: kept alive, their nodes would
-    hold on to the stream they were built on and to what they saved."""
-    from torch.utils._pytree import tree_map
-
-    return tree_map(lambda t: t.detach() if isinstance(t, torch.Tensor) else t, outputs)
-
-
 class CapturedStep:
     """``step_fn(*static_inputs)`` (zero_grad, forward, loss, backward, optimizer.step) captured once
     after ``warmup`` eager iterations on a side stream, then replayed by ``__call__``.
@@ -86,7 +78,7 @@ class CapturedStep:
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s), capture_warmup():
             for _ in range(max(1, warmup)):  # real steps: allocator warm-up, first-step optimizer state
-                self.warmup_outputs = _detached(self.step_fn(*self.static_inputs))
+                self.warmup_outputs = self.step_fn(*self.static_inputs)
         torch.cuda.current_stream().wait_stream(s)
         from ..ops.act import step_counter
 
@@ -102,8 +94,9 @@ class CapturedStep:
 
         from ..ops import wcache
 
-        with suspend_polling(), wcache.step_capture(), torch.cuda.graph(self.graph, stream=s):  # no event queries mid-capture
-            self.outputs = _detached(self.step_fn(*self.static_inputs))
+        self._operands = wcache.step_capture([p for g in self.opt.param_groups for p in g["params"]])
+        with suspend_polling(), self._operands, torch.cuda.graph(self.graph, stream=s):  # no event queries mid-capture
+            self.outputs = self.step_fn(*self.static_inputs)
         # the capture executed nothing: undo its host-side bookkeeping
         for f, h in zip(self.opt._flat, host):
             if f is not None:
@@ -111,6 +104,15 @@ class CapturedStep:
         self._counted = [m for m in self._bns if m.__dict__.get("_dv_nbt_pending", 0) != pending[id(m)]]
         for m in self._counted:
             m._dv_nbt_pending = pending[id(m)]
+
+    def release(self):
+        """Keep the outputs without their autograd graphs, which backward has used up. Alive, their nodes hold on to
+        the stream they were built on, and an operator that looks for live graphs of a parameter
+        (ops.common.track_leaves) refuses to be captured on another: the next signature's."""
+        from torch.utils._pytree import tree_map
+
+        self.outputs, self.warmup_outputs = tree_map(
+            lambda t: t.detach() if isinstance(t, torch.Tensor) else t, (self.outputs, self.warmup_outputs))
 
     def __call__(self, *inputs):
         for dst, src in zip(self.static_inputs, inputs):
@@ -125,6 +127,7 @@ class CapturedStep:
 
         advance_dropout_step()  # fresh dropout masks per replay (ops/act.py)
         self.graph.replay()
+        self._operands.replayed()
         return self.outputs
 
 
@@ -205,5 +208,6 @@ class GraphedTrainStep:
             return loss, extra
 
         cap = CapturedStep(step_fn, opt, static, model=ddp.module if ddp is not None else self.model, warmup=1)
+        cap.release()
         self.graphs[sig] = (cap, spec)
         return cap.warmup_outputs

@@ -335,7 +335,7 @@ class _FlatOptimizer(torch.optim.Optimizer):
         if any(f is not None and f["param"].is_cuda for f in self._flat):
             from ..ops import wcache
 
-            wcache.after_step()  # one batched re-layout of every cached bf16 weight operand
+            wcache.after_step(owner=self)  # one batched re-layout of every cached bf16 weight operand
         return loss
 
     def _update(self, group, f, off, n, gs):  # pragma: no cover - abstract

@@ -184,7 +184,7 @@ class Fake:
 
 
 def test_every_signature_is_captured_beside_the_outputs_of_the_others(on_cpu, monkeypatch):
-    """Each capture has a stream of its own; a step that returns its loss as it is leaves no graph behind."""
+    """Each capture has a stream of its own; a step that returns its loss as it is leaves no graph behind, once released."""
     import contextlib
 
     from deep_vision_amd.ops import act
@@ -215,6 +215,7 @@ def test_every_signature_is_captured_beside_the_outputs_of_the_others(on_cpu, mo
     kept = []
     for rows in (4, 3, 2):
         kept.append(CapturedStep(step, opt, (torch.randn(rows, 8).bfloat16(), torch.zeros(rows, dtype=torch.int64)), warmup=1))
+        kept[-1].release()
     for cap in kept:
         assert cap.outputs[0].grad_fn is None and cap.warmup_outputs[1]["again"][0].grad_fn is None
         assert cap.outputs[1]["again"][1] == 3
