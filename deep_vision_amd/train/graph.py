@@ -35,6 +35,20 @@ from typing import Callable, Sequence
 import torch
 
 
+RETIRE_SECONDS = 0.35
+
+
+def retire_collectives():
+    """Give ProcessGroupNCCL's watchdog thread the time to find the finished collectives of the eager steps. It looks at
+    its list every tenth of a second and queries an event for each entry; a query during a capture is an error
+    that ends the process. (The captured collectives are not on the list.)"""
+    import time
+
+    if torch.distributed.is_available() and torch.distributed.is_initialized() \
+            and torch.distributed.get_backend() == "nccl":
+        time.sleep(RETIRE_SECONDS)
+
+
 class CapturedStep:
     """``step_fn(*static_inputs)`` (zero_grad, forward, loss, backward, optimizer.step) captured once
     after ``warmup`` eager iterations on a side stream, then replayed by ``__call__``.
@@ -84,6 +98,7 @@ class CapturedStep:
 
         step_counter(torch.cuda.current_device())  # exists before the capture (captured dropouts read it)
         torch.cuda.synchronize()
+        retire_collectives()
         self.opt.use_device_hparams(True)
         host = [(f["step"], f["first"]) if f else None for f in self.opt._flat]
         pending = {id(m): m.__dict__.get("_dv_nbt_pending", 0) for m in self._bns}

@@ -183,25 +183,52 @@ class Fake:
         return lambda *args: None
 
 
-def test_every_signature_is_captured_beside_the_outputs_of_the_others(on_cpu, monkeypatch):
-    """Each capture has a stream of its own; a step that returns its loss as it is leaves no graph behind, once released."""
+@pytest.fixture
+def captures(on_cpu, monkeypatch):
+    """CapturedStep on CPU tensors; the list of what it does to the device, in order."""
     import contextlib
 
     from deep_vision_amd.ops import act
-    from deep_vision_amd.train.graph import CapturedStep
+
+    done = []
 
     @contextlib.contextmanager
     def within(stream, capturing=False):
         old = dict(on_cpu)
         on_cpu.update(stream=stream.handle, capturing=capturing)
+        done.append("capture" if capturing else "warm-up")
         yield
         on_cpu.update(old)
 
-    for name, to in (("Stream", Fake), ("CUDAGraph", Fake), ("current_stream", Fake), ("synchronize", lambda: None),
-                     ("current_device", lambda: 0), ("stream", within),
-                     ("graph", lambda g, stream: within(stream, True))):
+    for name, to in (("Stream", Fake), ("CUDAGraph", Fake), ("current_stream", Fake),
+                     ("synchronize", lambda: done.append("synchronize")), ("current_device", lambda: 0),
+                     ("stream", within), ("graph", lambda g, stream: within(stream, True))):
         monkeypatch.setattr(torch.cuda, name, to)
     monkeypatch.setattr(act, "step_counter", lambda dev: None)
+    return done
+
+
+@pytest.mark.parametrize("backend", ["nccl", None])
+def test_a_capture_begins_when_the_collectives_before_it_are_off_the_watchdogs_list(captures, monkeypatch, backend):
+    import time
+
+    from deep_vision_amd.train.graph import CapturedStep
+
+    monkeypatch.setenv("TORCH_NCCL_ASYNC_ERROR_HANDLING", "0")
+    monkeypatch.setattr(torch.distributed, "is_initialized", lambda: backend is not None)
+    monkeypatch.setattr(torch.distributed, "get_backend", lambda: backend)
+    monkeypatch.setattr(time, "sleep", lambda s: captures.append(s))
+    opt = FusedSGD([torch.nn.Parameter(torch.zeros(3))], lr=0.1)
+    CapturedStep(lambda: None, opt)
+    waits = [x for x in captures if isinstance(x, float)]
+    assert captures == ["warm-up", "synchronize", *waits, "capture"]
+    assert (sum(waits) > 0.2) if backend else not waits  # the watchdog's period is 0.1 s
+
+
+def test_every_signature_is_captured_beside_the_outputs_of_the_others(captures):
+    """Each capture has a stream of its own; a step that returns its loss as it is leaves no graph behind, once released."""
+    from deep_vision_amd.train.graph import CapturedStep
+
     norm_layer, fc = head()
     opt = FusedSGD([*norm_layer.parameters(), *fc.parameters()], lr=0.1)
 
