@@ -273,7 +273,7 @@ struct DvXent {
   const float* go;         // backward: the upstream gradient, [N] for DV_XENT_NONE, else [1]
   const float* total;      // backward, mean: [1] is the number of rows that count
 };
-int64_t dv_linear_xent_fwd_bytes(const DvXent& a);
+int64_t dv_linear_xent_fwd_bytes(const DvXent& a);  // -1: more tiles than a launch holds
 int64_t dv_linear_xent_bwd_bytes(const DvXent& a, int need_x, int need_w, int need_b);
 // lse [N][2] (backward's; largest logit, log2 of the sum above it) and loss_rows [N] may be null; out (the reduced loss) and total [2] go together, null for DV_XENT_NONE
 int dv_linear_xent_fwd(const DvXent& a, void* ws, float* lse, float* loss_rows, float* total, float* out, hipStream_t st);

@@ -590,11 +590,16 @@ Plan plan_form(int f, int64_t M, int64_t N, int ktiles, bool may_split, Ends end
   }
   return best;
 }
+// a launch holds less than 2^32 threads
+bool fits(int f, int64_t M, int64_t N) {
+  constexpr int THREADS[FORMS] = {Big::NTHREADS, Mid::NTHREADS, Small::NTHREADS, Thin::NTHREADS};
+  return (int64_t)cdiv(M, FORM_M[f]) * cdiv(N, FORM_N[f]) * THREADS[f] < 1LL << 32;
+}
 Plan plan(int64_t M, int64_t N, int ktiles, Ends ends) {
   Plan best = plan_form(0, M, N, ktiles, false, ends);
   for (int f = 1; f < FORMS; ++f) {
     const Plan p = plan_form(f, M, N, ktiles, false, ends);
-    if (p.us < best.us) best = p;
+    if (p.us < best.us && fits(f, M, N)) best = p;
   }
   return best;
 }
@@ -704,7 +709,10 @@ void launch_reduce(const DvXent& a, const OutArgs& g, hipStream_t st) {
 }
 }  // namespace
 
-int64_t dv_linear_xent_fwd_bytes(const DvXent& a) { return fwd_layout(a).bytes; }
+int64_t dv_linear_xent_fwd_bytes(const DvXent& a) {
+  const FwdLayout l = fwd_layout(a);
+  return fits(l.p.form, a.V, a.N) ? l.bytes : -1;
+}
 int64_t dv_linear_xent_bwd_bytes(const DvXent& a, int need_x, int need_w, int need_b) {
   return bwd_layout(a, need_x, need_w, need_b).bytes;
 }
@@ -712,6 +720,7 @@ int64_t dv_linear_xent_bwd_bytes(const DvXent& a, int need_x, int need_w, int ne
 int dv_linear_xent_fwd(const DvXent& a, void* ws, float* lse, float* loss_rows, float* total, float* out, hipStream_t st) {
   if (!sane(a)) return -1;
   const FwdLayout l = fwd_layout(a);
+  if (!fits(l.p.form, a.V, a.N)) return -1;
   char* w = reinterpret_cast<char*>(ws);
   float2* part = reinterpret_cast<float2*>(w + l.part);
   float* psum = a.smooth > 0.f ? reinterpret_cast<float*>(w + l.psum) : nullptr;

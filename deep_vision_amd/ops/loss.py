@@ -128,7 +128,10 @@ def _linear_xent_forward(x, weight, bias, labels, smoothing, ignore_index, reduc
         wk = _operand(weight, Dp)
     b = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     args = _linear_xent_args(xk, wk, b, labels, V, Dp, D, ignore_index, smoothing, reduction)
-    ws = torch.empty(lib().linear_xent_fwd_bytes(*args), dtype=torch.uint8, device=dev)
+    need = lib().linear_xent_fwd_bytes(*args)
+    if need < 0:
+        raise ValueError(f"linear_cross_entropy: {N} rows against {V} classes are more than a call takes")
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
     # per row (largest logit, log2 of the sum above it); behind them (sum of the losses, rows that count)
     stats = torch.empty(2 * N + 2, dtype=F32, device=dev)
     loss = torch.empty(() if reduction else N, dtype=F32, device=dev)
@@ -196,8 +199,8 @@ def linear_cross_entropy(x, weight, labels, bias=None, label_smoothing=0.0, igno
     whatever x holds there. ``reduction`` is "mean" over the rows that count (0 if none does), "sum",
     or "none" (labels' shape). Products are summed in fp32, the loss and bias gradient are fp32, the
     gradient of the logits is rounded to bf16 for the two products behind it; the weight's gradient
-    has the weight's type and goes straight into a live ``.grad`` buffer. At most 2^22 rows and 2^30
-    classes."""
+    has the weight's type and goes straight into a live ``.grad`` buffer. At most 2^22 rows, 2^30 classes
+    and 2^38 logits."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:

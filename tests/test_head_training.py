@@ -420,3 +420,25 @@ def test_a_parameter_shared_by_two_streams():
             second = [F.linear_cross_entropy(x, fc.weight, y, fc.bias) for _ in range(2)]
         torch.cuda.synchronize()
         assert torch.equal(first, want) and all(torch.equal(t, want) for t in second)
+
+
+# ---------------------------------------------------------------- sizes
+def test_more_logits_than_a_launch_holds_are_refused(on_cpu):
+    on_cpu["kernels"].linear_xent_fwd_bytes = lambda *args: -1
+    _, fc = head()
+    with pytest.raises(ValueError, match="more than a call takes"):
+        call("linear_cross_entropy", None, fc, torch.randn(4, 8).bfloat16(), torch.zeros(4, dtype=torch.int64))
+    assert "linear_xent_fwd" not in on_cpu["kernels"].calls
+
+
+@gpu
+@pytest.mark.parametrize("rows,classes,fits", [(1 << 22, 1 << 16, True), (1 << 20, 1 << 18, True), (1 << 22, 1 << 18, False),
+                                               (1 << 20, 1 << 20, False), (1 << 22, 3, True), (1, 1 << 30, True), (256, 1 << 30, True),
+                                               (1 << 8, 1 << 29, True), (300, 1 << 30, False)])
+def test_which_sizes_a_launch_holds(rows, classes, fits):
+    """The sizes alone, nothing is launched: 2^32 threads are more than a launch takes, and the largest tile, 256 x 256,
+    has 512 of them. Few rows take larger tiles than they otherwise would."""
+    from deep_vision_amd._ext import lib
+
+    for D in (64, 2048):
+        assert (lib().linear_xent_fwd_bytes(0, D, 0, D, 0, 0, rows, classes, D, D, -100, 0.0, 1) >= 0) == fits

@@ -463,3 +463,42 @@ def test_two_streams_and_a_replayed_graph():
         torch.cuda.synchronize()
         loss, grads = run_and_check(nx, w, b, ny)
         assert torch.equal(loss, out[0]) and all(torch.equal(p, q) for p, q in zip(out[1], grads))
+
+
+@gpu
+def test_more_classes_than_a_launch_of_the_smallest_tiles_holds():
+    """2^28 classes in tiles of 32 x 32 would be 2^32 threads. A logit is off by (64 / 16 + 32) 2u sum|x w| (the module's
+    bound), some 1e-4; the gradients are held to 1 % of their norms (d is rounded to bf16, h = 0.4 %)."""
+    V, D, N = (1 << 28) + 5, 64, 3
+    g = torch.Generator(device=DEV).manual_seed(0)
+    w = torch.empty(V, D, dtype=BF16, device=DEV)
+    step = 1 << 24
+    for i in range(0, V, step):
+        n = min(step, V - i)
+        w[i:i + n] = torch.randn(n, D, generator=g, device=DEV).mul_(0.2)
+    x = torch.randn(N, D, generator=g, device=DEV).to(BF16).requires_grad_()
+    y = torch.tensor([V - 1, 0, 1 << 27], device=DEV)
+    w.requires_grad_()
+    loss = F.linear_cross_entropy(x, w, y, reduction="sum")
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    with torch.no_grad():
+        lse, chosen = torch.full((N,), -float("inf"), dtype=torch.float64, device=DEV), torch.zeros(N, dtype=torch.float64, device=DEV)
+        for i in range(0, V, step):
+            l = (x.float() @ w[i:i + step].float().t()).double()
+            lse = torch.logaddexp(lse, torch.logsumexp(l, 1))
+            for n in range(N):
+                if i <= y[n] < i + step:
+                    chosen[n] = l[n, y[n] - i]
+        assert abs(loss.item() - (lse - chosen).sum().item()) < 1e-3
+        want = torch.zeros(N, D, dtype=torch.float64, device=DEV)
+        for i in range(0, V, step):
+            part = w[i:i + step].float()
+            d = torch.exp((x.float() @ part.t()).double() - lse[:, None])
+            for n in range(N):
+                if i <= y[n] < i + step:
+                    d[n, y[n] - i] -= 1
+            want += (d.float() @ part).double()
+            if i + step >= V or i == 0:
+                rows = d.t() @ x.double()
+                assert (dw[i:i + step].double() - rows).norm() < 1e-2 * rows.norm()
+        assert (dx.double() - want).norm() < 1e-2 * want.norm()
