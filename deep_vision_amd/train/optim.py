@@ -536,6 +536,27 @@ class FusedAdamW(_FlatOptimizer):
             return super()._save_state(f, i, shape)
         return {name: t.clone() for name, t in self._slices(f, i).items()}
 
+    def load_state_dict(self, state_dict):
+        self._check_packed(state_dict["state"])
+        super().load_state_dict(state_dict)
+
+    def _check_packed(self, state):
+        """Refuse 8-bit states of tensors of other sizes, before any is loaded (one look at the device for all)."""
+        sizes, ends = [n for f in self._flat if f is not None for _, n in f["offsets"]], {}
+        for idx, n in enumerate(sizes):
+            st = state.get(idx, state.get(str(idx))) or {}
+            if "exp_avg_root" not in st:
+                continue
+            blocks = -(-n // self.BLOCK)
+            for k in ("exp_avg", "exp_avg_root", "exp_avg_scale", "exp_avg_root_scale"):
+                want = blocks if k.endswith("_scale") else blocks * self.BLOCK
+                if st[k].numel() != want:
+                    raise ValueError(f"FusedAdamW: {k} of a saved 8-bit state has {st[k].numel()} entries, expected {want}")
+                if want > n and not k.endswith("_scale"):
+                    ends.setdefault(st[k].device, []).append(st[k].reshape(-1)[n:].view(torch.uint8))
+        if any((torch.cat(t) & 0x7F).any() for t in ends.values()):
+            raise ValueError("FusedAdamW: a saved 8-bit state goes on behind its tensor's end: it is of a larger one")
+
     def _load_state(self, f, i, st):
         n = f["offsets"][i][1]
         packed = "exp_avg_root" in st
@@ -548,10 +569,6 @@ class FusedAdamW(_FlatOptimizer):
         mine = self._slices(f, i)
         for name in ("exp_avg", "exp_avg_root"):
             if packed:
-                for k in (name, name + "_scale"):
-                    if st[k].numel() != mine[k].numel():
-                        raise ValueError(f"FusedAdamW: {k} of a saved 8-bit state has {st[k].numel()} entries, "
-                                         f"expected {mine[k].numel()}")
                 mine[name].view(torch.uint8).copy_(st[name].contiguous().view(torch.uint8))
                 mine[name + "_scale"].copy_(st[name + "_scale"])
             elif "exp_avg" in st and "exp_avg_sq" in st:  # 32-bit moments: rounded to nearest, once

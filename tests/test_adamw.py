@@ -447,3 +447,19 @@ def test_8_bit_second_moment_settles_above_its_mean(b2):
     r = s["exp_avg_root"].float().view(-1, 256) * s["exp_avg_root_scale"][:, None]
     assert 0.01 < (r ** 2).mean() / v.mean() - 1 < 0.13
     assert -0.01 < r.mean() / v.sqrt().mean() - 1 < 0.07  # the mean of roots moves by no more than half of that
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_saved_8_bit_state_of_another_size_is_refused(bits):
+    """More or fewer blocks, and a longer tensor of as many blocks, whose codes go on behind the shorter one's end."""
+    _, saved = make("cpu", 8, sizes=[600])
+    feed(saved.param_groups[0]["params"], 0)
+    saved.step()
+    state = saved.state_dict()
+    for n, text in ((500, "expected 512"), (800, "expected 1024"), (599, "of a larger one")):
+        with pytest.raises(ValueError, match=text):
+            make("cpu", bits, sizes=[n])[1].load_state_dict(state)
+    opt = make("cpu", bits, sizes=[600])[1]
+    state["state"][0]["exp_avg"].view(torch.uint8)[600:] = 0x80  # zeros with a sign
+    opt.load_state_dict(state)
+    assert opt._flat[0]["step"] == 1
