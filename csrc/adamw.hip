@@ -5,7 +5,7 @@
 //
 // Bound by memory: 28 bytes a value with 32-bit moments (p, m, v read and written, g read), 16 with
 // 8-bit ones. Measured, moments, gradients and parameters out of cache: 25.6M values 123 us with 32-bit
-// moments (5.8 TB/s of those bytes), 86 us with 8-bit ones (4.8); 138M values in 8 bits 428 us (5.2; the
+// moments (5.8 TB/s of those bytes), 84 us with 8-bit ones (4.9); 138M values in 8 bits 430 us (5.1; the
 // non-temporal policy made that 445).
 //
 // 8-bit moments: m and r = sqrt(v) are held as e4m3 codes (the type torch calls float8_e4m3fn)

@@ -19,7 +19,9 @@
 // forward 70 us (5.9), backward 130 and 5 (4.6). Non-temporal stores of y or dx gain nothing where the
 // next operator reads them.
 //
-// Rows wider than 16384 columns are walked in a loop (three passes, the later ones from L2).
+// Rows wider than 16384 columns are walked in a loop of 2- or 4-byte loads, three passes forward and two
+// backward, the later ones from cache, and the parameter sums in a launch of their own: 1024 x 20000 bf16 forward
+// 41 us (2.0 TB/s), backward 38 + 21 and 5 for the fold. No model here has such rows; they are right, not fast.
 #include "common.h"
 #include "kernels.h"
 

@@ -23,9 +23,11 @@
 //  * sums that split an axis go through fp32 slabs added in a fixed order: no atomics, the same bits
 //    every time.
 //
-// Measured: 8192 rows x 65536 classes x 2048 wide 6.9 ms: the statistics 1.79 (1.23 PFLOP/s), d 1.99 (1.10: its
-// 1 GB of stores is not hidden), dx and dw 3.28 (1.34). 771 x 20011 x 1021 245 us: packing 16, statistics 52,
-// d 62, dx and dw 94 + 7 (670 TFLOP/s, 128 x 128 tiles). 256 x 1000 x 2048: 10 + 5, 12, 12.5 us in 32 x 32 and 64 x 64.
+// Measured, bf16 weight and no bias: 8192 rows x 65536 classes x 2048 wide 6.9 to 7.1 ms from box to box: the statistics
+// 1.73 (1.27 PFLOP/s), d 1.92 (1.14: its 1 GB of stores is not hidden), dx and dw 3.21 (1.37). 771 x 20011 x 1021
+// 245 us: packing 16, statistics 52, d 62, dx and dw 94 + 7 (670 TFLOP/s, 128 x 128 tiles). 256 x 1000 x 2048: 9 + 5, 12,
+// 12 us in 32 x 32 and 64 x 64. An fp32 parameter whose gradient is added into its buffer: 7.1 ms, 253 us; a bias costs
+// 8192 x 65536 another 0.3 ms.
 #include "gemm_tile.h"
 #include "kernels.h"
 
@@ -567,9 +569,8 @@ __global__ __launch_bounds__(256) void pack_kernel(DvPack m0, DvPack m1, int b0)
 
 // ------------------------------------------------------------------------------------------- host
 // Tile and split of an M x N x (64 ktiles) product: the least time by a model of a K-tile's time on a full
-// CU (throughput) and alone (latency) and of a block's ends, its constants fitted to measurements. Over
-// 1 .. 8192 rows, 64 .. 65536 classes and widths of 64 .. 2500 (88 shapes) the form it takes is within 8 % of
-// the best, within 3 % for nine in ten.
+// CU (throughput) and alone (latency) and of a block's ends, its constants fitted to times of these kernels at
+// 1 .. 8192 rows, 64 .. 65536 classes and widths of 64 .. 2500.
 struct Plan { int form, splits; double us; };
 constexpr int FORMS = 4, OUT_FORMS = 3, FORM_M[FORMS] = {256, 128, 64, 32}, FORM_N[FORMS] = {256, 128, 64, 32};
 enum Ends { STATS, GRAD, OUT };  // what a block does behind its sums
