@@ -68,6 +68,8 @@ def _settle():
     valid, others of its parameters were laid out before the last steps. (A version or an address that has
     changed is not taken over: such an entry is laid out anew.)"""
     global _replayed
+    if not _replayed:
+        return
     graphs, _replayed = list(_replayed.values()), {}
     for k, e in list(_entries.items()):
         p = e[0]()
@@ -96,7 +98,7 @@ def get(param, G, pad, mode, compute, Sp=0):
     mode 2 = the forward layout with the filter width padded to ``Sp`` (tap-packed stem)."""
     if not ENABLED:
         return compute(None)
-    if _replayed:
+    if _replayed:  # (the call itself costs as much as a hit)
         _settle()
     k = _key(param, G, pad, mode, Sp)
     e = _entries.get(k)
