@@ -267,19 +267,23 @@ def track_leaves(ctx, *leaves):
 
 
 def updates_seen(t):
-    """What ``refuse_updated`` needs of a tensor that a backward pass is going to read again: the update count
+    """What ``refuse_updated`` needs of a tensor that a backward pass is going to read again: the update counts
     of the parameter it is, or is a view of (train.optim counts), or None."""
     if t is None:
         return None
-    count = getattr(t if t._base is None else t._base, "_dv_updates", None)
-    return None if count is None else (count, count[0], t.data_ptr())
+    counts = getattr(t if t._base is None else t._base, "_dv_updates", None)
+    return None if counts is None else (counts, counts[0][0], counts[1][0], t.data_ptr())
 
 
 def refuse_updated(what, name, t, seen):
-    """Raise where an optimizer has moved ``t`` since ``updates_seen(t)``. The fused optimizers write through raw
+    """Raise where an optimizer has moved ``t`` since ``seen = updates_seen(t)``. The fused optimizers write through raw
     pointers, which autograd's own check of saved tensors cannot notice. (A tensor that saved-tensor hooks
     brought back from elsewhere still holds what the forward pass saw.)"""
-    if seen is not None and seen[0][0] != seen[1] and (t.data_ptr() == seen[2] or getattr(t, "_dv_updates", None) is seen[0]):
+    if seen is None:
+        return
+    counts, own, group, at = seen
+    moved = counts[0][0] != own or counts[1][0] != group
+    if moved and (t.data_ptr() == at or getattr(t, "_dv_updates", (None,))[0] is counts[0]):
         raise RuntimeError(f"{what}: an optimizer has updated the {name} since the forward pass, whose results the gradients "
                            "need: call backward() before step()")
 

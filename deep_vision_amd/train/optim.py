@@ -103,10 +103,7 @@ class _FlatOptimizer(torch.optim.Optimizer):
                 p._dv_off = off
         f = dict(param=pflat, grad=gflat, views=views, gviews=gviews, offsets=offs, step=0, first=True, shared=shared)
         f["ptrs"] = [v.data_ptr() for v in views]
-        for p in ps:
-            if not hasattr(p, "_dv_updates"):
-                p._dv_updates = [0]
-        f["updates"] = [p._dv_updates for p in ps]
+        self._share_count(f, ps)
         f["states"] = self._new_states(f)
         if old is not None:  # re-bound after the parameters moved: carry the optimizer state over
             f["step"], f["first"] = old["step"], old["first"]
@@ -194,14 +191,27 @@ class _FlatOptimizer(torch.optim.Optimizer):
             self._write_hp(group, f)
 
     @staticmethod
+    def _share_count(f, ps):
+        """Give each parameter its update counts, (of its own, of the group's whole steps): the kernels write through raw
+        pointers, so a backward pass that reads a parameter again cannot tell from its version
+        (ops.common.refuse_updated). A parameter that comes from another group (the third entry: their own
+        counts) counts whole steps on its own too, for the passes that remember the other group's."""
+        old = [getattr(p, "_dv_updates", None) for p in ps]
+        group = old[0][1] if old[0] is not None else None
+        if group is None or group[1] != len(ps) or any(c is None or c[1] is not group for c in old):
+            group = [0, len(ps), [c[0] for c in old if c is not None]]
+            for p, c in zip(ps, old):
+                p._dv_updates = ([0] if c is None else c[0], group)
+        f["count"], f["counts"] = group, [p._dv_updates[0] for p in ps]
+
+    @staticmethod
     def _count_updates(f, segs):
-        """Count the update of each parameter in the segments ``segs``: the kernels write through raw pointers, so a
-        backward pass that reads a parameter again cannot tell from its version (ops.common.refuse_updated)."""
         if len(segs) == 1 and segs[0][1] == f["param"].numel():
-            for count in f["updates"]:
+            f["count"][0] += 1
+            for count in f["count"][2]:
                 count[0] += 1
             return
-        for count, (at, n) in zip(f["updates"], f["offsets"]):
+        for count, (at, n) in zip(f["counts"], f["offsets"]):
             if any(off <= at and at + n <= off + k for off, k in segs):
                 count[0] += 1
 

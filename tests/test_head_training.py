@@ -96,6 +96,32 @@ def test_a_step_of_the_bias_alone_or_of_neither(on_cpu):
         out.sum().backward()
 
 
+@pytest.mark.parametrize("move", ["again", "split", "joined"])
+def test_a_step_of_an_optimizer_made_between_the_passes(on_cpu, move):
+    """The parameters move from one optimizer's buffer to others' between the passes; what steps then counts, and
+    what does not step does not."""
+    norm_layer, fc = head()
+    x, y = torch.randn(4, 8).bfloat16().requires_grad_(), torch.zeros(4, dtype=torch.int64)
+    params = [*fc.parameters(), *norm_layer.parameters()]
+    if move == "joined":
+        FusedSGD(fc.parameters(), lr=0.1), FusedSGD(norm_layer.parameters(), lr=0.1)
+    else:
+        FusedSGD(params, lr=0.1)
+    for stepped in (True, False):
+        out = call("linear_cross_entropy", None, fc, x, y)
+        if move == "split":
+            opt, other = FusedSGD(fc.parameters(), lr=0.1), FusedSGD(norm_layer.parameters(), lr=0.1)
+        else:
+            opt, other = FusedSGD(params, lr=0.1), FusedSGD([torch.nn.Parameter(torch.ones(2))], lr=0.1)
+        other.step()
+        if stepped:
+            FusedSGD(opt.param_groups[0]["params"], lr=0.1).step()  # the same parameters once more
+            with pytest.raises(RuntimeError, match="an optimizer has updated"):
+                out.sum().backward()
+        else:
+            out.sum().backward()
+
+
 @gpu
 @pytest.mark.parametrize("op", ["layer_norm", "linear_cross_entropy"])
 def test_a_step_between_the_passes_is_refused_on_the_gpu(op):
