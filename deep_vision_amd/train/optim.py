@@ -30,6 +30,11 @@ class _FlatOptimizer(torch.optim.Optimizer):
         for group in self.param_groups:
             self._flat.append(self._flatten_group(group))
 
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        if hasattr(self, "_flat"):  # behind __init__, which flattens its groups itself
+            self._flat.append(self._flatten_group(self.param_groups[-1]))
+
     # ---------------- flat storage ----------------
     @staticmethod
     def _shared_span(ps, sizes):

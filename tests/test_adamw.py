@@ -463,3 +463,23 @@ def test_a_saved_8_bit_state_of_another_size_is_refused(bits):
     state["state"][0]["exp_avg"].view(torch.uint8)[600:] = 0x80  # zeros with a sign
     opt.load_state_dict(state)
     assert opt._flat[0]["step"] == 1
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param(DEV, marks=gpu)])
+@pytest.mark.parametrize("name,kw", [("AdamW", {}), ("AdamW", {"state_bits": 8}), ("Adam", {}), ("SGD", {"momentum": 0.9}),
+                                     ("RMSprop", {})])
+def test_a_group_added_later_moves_as_from_the_start(dev, name, kw):
+    sizes = [300, 7]
+    a, b = ([torch.nn.Parameter(t) for t in tensors(sizes, dev)] for _ in range(2))
+    whole = OPTIMIZERS[name]([{"params": a[:1]}, {"params": a[1:], "lr": 0.05}], lr=0.01, **kw)
+    added = OPTIMIZERS[name](b[:1], lr=0.01, **kw)
+    added.add_param_group({"params": b[1:], "lr": 0.05})
+    for step in range(3):
+        for ps, opt in ((a, whole), (b, added)):
+            feed(ps, step)
+            opt.step()
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and not torch.equal(a[1].cpu(), tensors(sizes)[1])
+    again = OPTIMIZERS[name]([{"params": [torch.nn.Parameter(torch.zeros(300))]}, {"params": [torch.nn.Parameter(torch.zeros(7))]}],
+                             lr=0.01, **kw)
+    again.load_state_dict(added.state_dict())
+    assert [f["step"] for f in again._flat] == [3, 3]
