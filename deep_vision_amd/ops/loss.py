@@ -200,7 +200,8 @@ def linear_cross_entropy(x, weight, labels, bias=None, label_smoothing=0.0, igno
     or "none" (labels' shape). Products are summed in fp32, the loss and bias gradient are fp32, the
     gradient of the logits is rounded to bf16 for the two products behind it; the weight's gradient
     has the weight's type and goes straight into a live ``.grad`` buffer. At most 2^22 rows, 2^30 classes
-    and 2^38 logits."""
+    and 2^38 logits. As for ``linear``, the operand of a parameter follows its in-place changes and the fused
+    optimizers; what is written through ``.data`` shows from the next step on (or behind ``ops.wcache.clear()``)."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:

@@ -47,16 +47,28 @@ class step_capture:
         self.laid = {k: (_entries[k][1], _entries[k][0]().data_ptr()) for k in keys}
         if devices:
             self.table = _make_table(keys, devices.pop())
+        self.version = self._version()
         _captures.append(self)
         return self
+
+    def _version(self):
+        return sum([p._version for p in self.params.values()])
 
     def __exit__(self, *exc):
         _captures.remove(self)
 
     def refresh(self):
-        """Record the launch that lays out every operand anew."""
+        """Launch, or record, what lays out every operand anew."""
         if self.table is not None:
             lib().wprep_batched(ptr(self.table[0]), ptr(self.table[1]), self.table[2], stream_handle())
+
+    def catch_up(self):
+        """Before a replay: parameters that torch operations have changed since (a loaded checkpoint) are laid out anew,
+        as the graph's own forward pass only reads the operands."""
+        version = self._version()
+        if version != self.version:
+            self.version = version
+            self.refresh()
 
     def replayed(self):
         """The graph has been launched: the operands it refreshes are those of the new parameters."""

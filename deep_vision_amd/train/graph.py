@@ -141,6 +141,7 @@ class CapturedStep:
         from ..ops.act import advance_dropout_step
 
         advance_dropout_step()  # fresh dropout masks per replay (ops/act.py)
+        self._operands.catch_up()
         self.graph.replay()
         self._operands.replayed()
         return self.outputs

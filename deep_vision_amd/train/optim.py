@@ -270,7 +270,8 @@ class _FlatOptimizer(torch.optim.Optimizer):
         return [f["grad"] for f in self._flat if f]
 
     def flat_params(self):
-        """Each group's parameters as the one flat fp32 buffer the update runs over."""
+        """Each group's parameters as the one flat fp32 buffer the update runs over, to be read: what is written to it
+        passes by autograd's versions and the cached operands (ops/wcache.py)."""
         return [f["param"] for f in self._flat if f]
 
     def flat_states(self):

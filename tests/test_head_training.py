@@ -468,3 +468,38 @@ def test_which_sizes_a_launch_holds(rows, classes, fits):
 
     for D in (64, 2048):
         assert (lib().linear_xent_fwd_bytes(0, D, 0, D, 0, 0, rows, classes, D, D, -100, 0.0, 1) >= 0) == fits
+
+
+@gpu
+def test_a_checkpoint_loaded_between_replays_of_a_training_step():
+    """The next replay starts from the loaded parameters, as an eager step does."""
+    from deep_vision_amd.train.graph import CapturedStep
+
+    def make():
+        norm_layer, fc = head(64, 200, DEV)
+        model = torch.nn.Sequential(norm_layer, fc)
+        opt = FusedSGD(model.parameters(), lr=0.1)
+
+        def step(x, y):
+            opt.zero_grad()
+            loss = F.linear_cross_entropy(norm_layer(x), fc.weight, y, fc.bias)
+            loss.backward()
+            opt.step()
+            return loss.detach()
+
+        return model, opt, step
+
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x, y = torch.randn(48, 64, generator=g, device=DEV).bfloat16(), torch.randint(0, 200, (48,), generator=g, device=DEV)
+    model, opt, step = make()
+    twin, _, eager = make()
+    saved = {k: v + 0.5 * torch.randn(v.shape, generator=g, device=DEV) for k, v in model.state_dict().items()}
+    cap = CapturedStep(step, opt, (x, y), warmup=1)
+    eager(x, y)
+    for k in range(4):
+        if k % 2 == 0:
+            model.load_state_dict(saved), twin.load_state_dict(saved)
+        a, b = cap(x, y), eager(x, y)
+        torch.cuda.synchronize()
+        assert torch.equal(a, b), k
+        assert all(torch.equal(p, q) for p, q in zip(model.parameters(), twin.parameters())), k

@@ -210,3 +210,19 @@ def test_a_step_captured_by_hand(kernels, capture):
     with wcache.step_capture([q]), capture:  # a second optimizer in a captured step
         wcache.after_step(CPU, owner)
     assert kernels.refreshed == 1 and len(kernels.single) == 2
+
+
+def test_parameters_changed_between_replays_are_laid_out_before_the_next(kernels, capture):
+    p = torch.nn.Parameter(torch.zeros(4, 8))
+    lay(p)
+    step = wcache.step_capture([p])
+    with step, capture:
+        wcache.after_step(CPU)
+    assert kernels.refreshed == 1
+    for change, launches in ((False, 1), (True, 2), (False, 2), (True, 3)):
+        if change:
+            with torch.no_grad():
+                p.mul_(0.5)
+        step.catch_up()
+        step.replayed()
+        assert kernels.refreshed == launches
