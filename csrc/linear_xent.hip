@@ -23,7 +23,7 @@
 //  * sums that split an axis go through fp32 slabs added in a fixed order: no atomics, the same bits
 //    every time.
 //
-// Measured, bf16 weight and no bias: 8192 rows x 65536 classes x 2048 wide 6.9 to 7.1 ms from box to box: the statistics
+// Measured, bf16 weight and no bias: 8192 rows x 65536 classes x 2048 wide 6.9 to 7.1 ms from machine to machine: the statistics
 // 1.73 (1.27 PFLOP/s), d 1.92 (1.14: its 1 GB of stores is not hidden), dx and dw 3.21 (1.37). 771 x 20011 x 1021
 // 245 us: packing 16, statistics 52, d 62, dx and dw 94 + 7 (670 TFLOP/s, 128 x 128 tiles). 256 x 1000 x 2048: 9 + 5, 12,
 // 12 us in 32 x 32 and 64 x 64. An fp32 parameter whose gradient is added into its buffer: 7.1 ms, 253 us; a bias costs

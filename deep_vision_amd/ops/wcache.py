@@ -9,6 +9,8 @@ Here each (parameter, layout) gets a persistent buffer:
 * the fused optimizers call ``after_step()`` once per step: the epoch advances and ONE batched
   kernel (csrc/elementwise.hip ``wprep_batched_kernel``) refreshes every registered buffer on the
   current stream, right after the parameter update -- so the next forward / backward only hit.
+* a captured training step refreshes its own parameters' buffers in every replay (``step_capture``);
+* a buffer that one stream laid out is waited for by the first use on another, until a step has refreshed it.
 """
 from __future__ import annotations
 
